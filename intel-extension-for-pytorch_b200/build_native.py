@@ -6,11 +6,13 @@ The shared library lands next to the Python package (ipex_b200/libwoq_b200.so) s
 travels with the source tree; nothing is installed into site-packages.
 """
 import argparse
+import concurrent.futures
 import hashlib
 import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -35,8 +37,9 @@ CUDA_SOURCES = [
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC", "-Xlinker", "-soname=libwoq_b200.so",
+    "-Xcompiler", "-fPIC", "--shared", "-Xlinker", "-soname=libwoq_b200.so",
 ]
+LINK_FLAGS = ("--shared", "-Xlinker", "-soname=libwoq_b200.so")
 
 
 def _nvcc():
@@ -67,12 +70,19 @@ def build(force=False, verbose=False):
     # link into a temporary name and rename: a process that has the old library mapped keeps its
     # own copy instead of seeing the file change under it
     tmp = LIB + ".new"
-    cmd += [os.path.join(CSRC, s) for s in CUDA_SOURCES] + ["-o", tmp]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed building libwoq_b200.so")
+
+    def run(args):
+        res = subprocess.run(args, capture_output=True, text=True)
+        if verbose or res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed building libwoq_b200.so")
+
+    with tempfile.TemporaryDirectory() as objects, concurrent.futures.ThreadPoolExecutor(os.cpu_count()) as pool:
+        objs = [os.path.join(objects, s + ".o") for s in CUDA_SOURCES]
+        compile_cmd = [a for a in cmd if a not in LINK_FLAGS] + ["-c"]
+        list(pool.map(run, [compile_cmd + [os.path.join(CSRC, s), "-o", o] for s, o in zip(CUDA_SOURCES, objs)]))
+        run(cmd + objs + ["-o", tmp])
     os.replace(tmp, LIB)
     open(STAMP, "w").write(digest)
     return LIB
