@@ -395,6 +395,13 @@ int woq_b200_rmsnorm_quant(const void* x, int64_t ldx, const void* gamma, float 
                            int32_t act_quant_mode, void* y, int64_t ldy, void* qa, void* sa, void* zpa,
                            void* stream);
 
+/* The same behind a residual: sum = bf16(x + r) (the residual stream's new value), y = the RMSNorm of sum, and y's
+ * codes, scales and zero points as above; y itself is not written.  `sum` may be x or r.  Rows of up to 131072
+ * elements (k a multiple of 16).  A row whose sum of squares is not finite gets the scale NaN. */
+int woq_b200_add_rmsnorm_quant(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* gamma, float eps,
+                               int64_t m, int64_t k, int32_t act_quant_mode, void* sum, int64_t lds, void* qa, void* sa,
+                               void* zpa, void* stream);
+
 /* woq_b200_linear on activations that are already quantised (by woq_b200_rmsnorm_quant, or taken
  * from woq_b200_int8_internals): codes qa [m, K], scales sa [m], zero points zpa [m] (null for the
  * symmetric mode).  The context must be on the tcgen05 INT8 route (INT8 weights, lowp INT8) with a
@@ -403,6 +410,64 @@ int woq_b200_rmsnorm_quant(const void* x, int64_t ldx, const void* gamma, float 
 int woq_b200_linear_prequant(const woq_b200_ctx* ctx, const void* qa, const void* sa, const void* zpa, int64_t m,
                              int32_t fusion, const void* const* others, int32_t n_others, void* y, int64_t ldy,
                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Paged 4-bit key/value cache -------------------------------------------------------------
+ * What stands between a decoder layer's q/k/v and output projections when keys and values are kept in 4 bits.
+ * No reference counterpart (its caches hold the activations' type).
+ *
+ * A cache is one buffer [num_pages][kv_heads][page_size / 16] of blocks; a block holds 16 tokens of one head:
+ * 8 D bytes of key codes, 8 D bytes of value codes (both in the order of the attention kernel's matrix fragments,
+ * csrc/woq_kv4_common.cuh), then {scale, lowest value} pairs of `dtype` for every token and group of group_size
+ * elements of the keys, then of the values.  With m = min x and s = (max x - m) / 15 rounded toward zero to `dtype`,
+ * code c = clamp(rint((x - m) / s), 0, 15) (0 where s is 0) stands for c * s + m, rounded once to `dtype`.
+ * A slot is page * page_size + position within the page. */
+typedef struct woq_b200_kv4_desc {
+  int64_t num_pages;
+  int32_t kv_heads;
+  int32_t head_dim;   /* D: 64, 128 or 256                          */
+  int32_t page_size;  /* tokens, a multiple of 16                   */
+  int32_t group_size; /* 32, 64 or 128, at most head_dim            */
+  int32_t dtype;      /* WOQ_B200_T_BF16 or _F16: of q, k, v as well */
+} woq_b200_kv4_desc;
+
+/* Bytes of the cache (0: not a valid description).  Any contents will do to start with: only slots that were
+ * appended to are looked at. */
+size_t woq_b200_kv4_bytes(const woq_b200_kv4_desc* desc);
+
+/* Rotates the first `rot` elements (a multiple of 16; 0: none) of every query and key head by its token's position,
+ * writes the queries to q_out [tokens][q_heads][D] and the quantised keys and values to the tokens' slots.
+ * Strides are in elements, multiples of 8; the elements of a head lie next to one another.  cos_sin: fp32
+ * [max_pos][rot], rot / 2 cosines then rot / 2 sines; pairs are (i, i + rot / 2), or (2 i, 2 i + 1) if `interleaved`.
+ * Rotated keys are rounded to `dtype` before they are quantised.  q may be null with q_heads 0.
+ * A slot outside the cache (-1 for padding) stores nothing; a position outside the table stores nothing either and
+ * makes the token's q_out NaN.  The slots of one call must be distinct.  Where a head's key or value has an element
+ * that is not finite, the key reads back as NaN (and scores NaN) and a value with such an element as zeros. */
+int woq_b200_kv4_append(const woq_b200_kv4_desc* desc, void* cache, const void* q, int64_t q_token_stride,
+                        int64_t q_head_stride, int32_t q_heads, const void* k, int64_t k_token_stride,
+                        int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                        const int64_t* slots, const int64_t* positions, const float* cos_sin, int64_t max_pos,
+                        int32_t rot, int32_t interleaved, int64_t tokens, void* q_out, void* stream);
+
+/* What the cache holds at `slots`: k, v [tokens][kv_heads][D] of `dtype`; zeros for slots outside the cache. */
+int woq_b200_kv4_read(const woq_b200_kv4_desc* desc, const void* cache, const int64_t* slots, int64_t tokens, void* k,
+                      void* v, void* stream);
+
+/* out = softmax(scale * q k^T) v over the cache.  Sequence b has seq_lens[b] cached tokens in the pages
+ * block_table[b][0], [1], .. (rows table_ld entries apart; lengths beyond max_pages pages are cut) and the query
+ * rows query_starts[b] .. query_starts[b + 1] - 1 (device array of batch + 1 entries; null: row b alone, and
+ * tokens == batch).  `causal`: its queries are its last tokens, and a query does not see the tokens after it.
+ * q_heads is a multiple of kv_heads; query head h reads kv head h / (q_heads / kv_heads).  A row that sees nothing is
+ * zeros; rows of `out` that belong to no sequence stay as they are.  Lengths, tables and starts are read on the
+ * device: a captured call follows them.  Workspace as for woq_b200_linear (its header zero before the first use).
+ * Keys of pages that the cache does not have are left out, and woq_b200_workspace_status then returns
+ * WOQ_B200_ERR_INVALID_ARG.  Two calls with the same arguments give the same bits. */
+size_t woq_b200_kv4_attention_workspace_bytes(const woq_b200_kv4_desc* desc, int64_t batch, int64_t tokens,
+                                              int32_t q_heads);
+int woq_b200_kv4_attention(const woq_b200_kv4_desc* desc, const void* cache, const void* q, int64_t q_token_stride,
+                           int64_t q_head_stride, int32_t q_heads, const int32_t* block_table, int64_t table_ld,
+                           int64_t max_pages, const int32_t* seq_lens, const int32_t* query_starts, int64_t batch,
+                           int64_t tokens, float scale, int32_t causal, void* out, int64_t out_token_stride,
+                           int64_t out_head_stride, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Parity hooks -------------------------------------------------------------------------
  * Dequantised weight [N, K] bf16 produced by the same device routine the tensor-core kernel
@@ -464,8 +529,9 @@ int woq_b200_pair_plan(int32_t weight_dtype, int32_t columns, int64_t tiles, int
 /* The token columns woq_b200_linear_grouped takes for groups of these many rows (a diagnostic; needs no GPU). */
 int woq_b200_grouped_columns(const int64_t* rows, int32_t groups, int32_t* columns);
 
-/* Reads the status word of a workspace (synchronises the stream).  WOQ_B200_OK, or
- * WOQ_B200_ERR_DEVICE_WAIT when a bounded wait inside a kernel gave up; the word is cleared. */
+/* Reads the status word of a workspace (synchronises the stream).  WOQ_B200_OK,
+ * WOQ_B200_ERR_DEVICE_WAIT when a bounded wait inside a kernel gave up, or WOQ_B200_ERR_INVALID_ARG when
+ * woq_b200_kv4_attention met a page that the cache does not have; the word is cleared. */
 int woq_b200_workspace_status(void* workspace, void* stream);
 
 #ifdef __cplusplus

@@ -33,6 +33,9 @@ CUDA_SOURCES = [
     "woq_moe.cu",
     "woq_i8_block_tc.cu",
     "woq_i8_pair.cu",
+    "woq_kv4.cu",
+    "woq_kv4_attend.cu",
+    "woq_kv4_capi.cu",
 ]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -21,6 +21,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <cmath>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -34,16 +35,17 @@ namespace {
 constexpr int64_t kHandleMagic = 0x574f5148414e444cll;  // "WOQHANDL"
 constexpr int64_t kGateUpStateBit = 0x100;                // pickled weight_dtype of a gate/up context
 
-int dtype_code(const at::Tensor& t) {
-  switch (t.scalar_type()) {
+int dtype_code_of(at::ScalarType t) {
+  switch (t) {
     case at::kFloat: return WOQ_B200_T_F32;
     case at::kHalf: return WOQ_B200_T_F16;
     case at::kBFloat16: return WOQ_B200_T_BF16;
     case at::kByte: return WOQ_B200_T_U8;
     case at::kChar: return WOQ_B200_T_S8;
-    default: TORCH_CHECK(false, "WOQ: unsupported tensor dtype ", t.scalar_type());
+    default: TORCH_CHECK(false, "WOQ: unsupported tensor dtype ", t);
   }
 }
+int dtype_code(const at::Tensor& t) { return dtype_code_of(t.scalar_type()); }
 
 #define WOQ_CHECK(expr)                                                       \
   do {                                                                        \
@@ -537,6 +539,169 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> woq_rmsnorm_quant(const at::Tenso
   return std::make_tuple(qa, sa, zpa);
 }
 
+// The same behind a residual: sum = bf16(input + residual), then woq_rmsnorm_quant of it.  Returns (sum, codes, scales,
+// zero points).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> woq_add_rmsnorm_quant(const at::Tensor& input,
+                                                                                 const at::Tensor& residual,
+                                                                                 const at::Tensor& weight, double eps,
+                                                                                 int64_t act_quant_mode) {
+  TORCH_CHECK(input.is_cuda() && input.scalar_type() == at::kBFloat16, "WOQ: add_rmsnorm_quant takes bf16 CUDA input");
+  TORCH_CHECK(residual.device() == input.device() && residual.scalar_type() == at::kBFloat16 &&
+                  residual.sizes() == input.sizes(),
+              "WOQ: the residual must be a bf16 tensor of the input's shape on its device");
+  TORCH_CHECK(input.dim() >= 1, "WOQ: add_rmsnorm_quant takes rows");
+  const int64_t K = input.size(-1);
+  TORCH_CHECK(weight.numel() == K, "WOQ: the norm weight has ", weight.numel(), " elements, expected ", K);
+  c10::cuda::CUDAGuard guard(input.device());
+  auto rows = [&](const at::Tensor& t) {
+    at::Tensor x = t.reshape({-1, K});
+    if (x.stride(-1) != 1 || x.stride(0) < K || (x.stride(0) % 8) != 0 || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15))
+      x = x.contiguous();
+    return x;
+  };
+  const at::Tensor x = rows(input), r = rows(residual);
+  at::Tensor g = weight.to(input.device(), at::kBFloat16).contiguous();
+  if (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15) g = g.clone();
+  const int64_t M = x.size(0);
+  at::Tensor sum = at::empty(input.sizes(), x.options());
+  at::Tensor qa = at::empty(input.sizes(), x.options().dtype(at::kChar));
+  at::Tensor sa = at::empty({M}, x.options().dtype(at::kFloat));
+  const bool asym = act_quant_mode == WOQ_B200_ACT_PER_M;
+  at::Tensor zpa = at::empty({asym ? M : 0}, x.options().dtype(at::kInt));
+  auto stream = at::cuda::getCurrentCUDAStream(input.get_device());
+  WOQ_CHECK(woq_b200_add_rmsnorm_quant(x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), g.data_ptr(),
+                                       static_cast<float>(eps), M, K, static_cast<int32_t>(act_quant_mode), sum.data_ptr(),
+                                       K, qa.data_ptr(), sa.data_ptr(), asym ? zpa.data_ptr() : nullptr, stream.stream()));
+  return std::make_tuple(sum, qa, sa, zpa);
+}
+
+// ---- paged 4-bit key/value cache ---------------------------------------------------------------
+// The cache is a uint8 tensor [pages, kv heads, page size / 16, block bytes]: its shape and the heads' width say the
+// group size (a block is 16 D codes in 16 D bytes and 128 bytes of parameters per group of a row).
+woq_b200_kv4_desc kv4_desc(const at::Tensor& cache, int64_t head_dim, at::ScalarType dtype) {
+  TORCH_CHECK(cache.is_cuda() && cache.scalar_type() == at::kByte && cache.dim() == 4 && cache.is_contiguous(),
+              "WOQ: the cache is a contiguous uint8 CUDA tensor [pages, kv heads, page size / 16, block bytes]");
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "WOQ: the 4-bit cache stands for bf16 or fp16 values, got ", dtype);
+  const int64_t params = cache.size(3) - 16 * head_dim;
+  TORCH_CHECK(params > 0 && params % 128 == 0 && (128 * head_dim) % params == 0, "WOQ: blocks of ", cache.size(3),
+              " bytes do not hold heads of ", head_dim, " elements");
+  TORCH_CHECK(cache.size(1) <= INT32_MAX && cache.size(2) <= INT32_MAX / 16 && head_dim <= 4096, "WOQ: cache shape out of range");
+  woq_b200_kv4_desc d{};
+  d.num_pages = cache.size(0);
+  d.kv_heads = static_cast<int32_t>(cache.size(1));
+  d.head_dim = static_cast<int32_t>(head_dim);
+  d.page_size = static_cast<int32_t>(cache.size(2) * 16);
+  d.group_size = static_cast<int32_t>(128 * head_dim / params);
+  d.dtype = dtype_code_of(dtype);
+  return d;
+}
+
+// [tokens, heads, D] with strides that the kernels take; a copy where it has others
+at::Tensor kv4_rows(const at::Tensor& t, const at::Tensor& cache, at::ScalarType dtype, const char* what) {
+  TORCH_CHECK(t.device() == cache.device() && t.scalar_type() == dtype && t.dim() == 3, "WOQ: ", what,
+              " must be [tokens, heads, head_dim] of ", dtype, " on the cache's device");
+  const bool fine = t.stride(2) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 &&
+                    (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  return fine ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+at::Tensor kv4_index(const at::Tensor& t, const at::Tensor& cache, at::ScalarType dtype, const char* what) {
+  TORCH_CHECK(t.device() == cache.device() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong), "WOQ: ", what,
+              " must be a tensor of int32 or int64 on the cache's device");
+  return t.to(dtype).contiguous();
+}
+
+at::Tensor kv4_cache_append(at::Tensor& cache, const at::Tensor& key, const at::Tensor& value, const at::Tensor& slots,
+                            const c10::optional<at::Tensor>& query, const c10::optional<at::Tensor>& positions,
+                            const c10::optional<at::Tensor>& cos_sin, bool interleaved) {
+  TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes(), "WOQ: key and value must be [tokens, kv heads, head_dim], both");
+  const auto dtype = key.scalar_type();
+  const woq_b200_kv4_desc d = kv4_desc(cache, key.size(2), dtype);
+  TORCH_CHECK(key.size(1) == d.kv_heads, "WOQ: key has ", key.size(1), " heads, the cache ", d.kv_heads);
+  const int64_t tokens = key.size(0);
+  c10::cuda::CUDAGuard guard(cache.device());
+  const at::Tensor k = kv4_rows(key, cache, dtype, "key"), v = kv4_rows(value, cache, dtype, "value");
+  const at::Tensor s = kv4_index(slots, cache, at::kLong, "slots");
+  TORCH_CHECK(s.dim() == 1 && s.size(0) == tokens, "WOQ: slots must have one entry per token");
+  at::Tensor q, q_out, pos, table;
+  const bool has_q = query.has_value() && query->defined();
+  if (has_q) {
+    q = kv4_rows(*query, cache, dtype, "query");
+    TORCH_CHECK(q.size(0) == tokens && q.size(2) == key.size(2), "WOQ: query must be [tokens, q heads, head_dim]");
+    TORCH_CHECK(q.size(1) >= 1 && q.size(1) <= 65535, "WOQ: the number of query heads is out of range");
+    q_out = at::empty(q.sizes(), key.options());
+  } else {
+    q_out = at::empty({0}, key.options());
+  }
+  int64_t rot = 0;
+  const bool turns = cos_sin.has_value() && cos_sin->defined();
+  TORCH_CHECK(turns == (positions.has_value() && positions->defined()), "WOQ: a rotation needs positions and cos_sin, both");
+  if (turns) {
+    TORCH_CHECK(cos_sin->device() == cache.device() && cos_sin->scalar_type() == at::kFloat && cos_sin->dim() == 2,
+                "WOQ: cos_sin must be fp32 [positions, rotated elements] on the cache's device");
+    table = cos_sin->contiguous();
+    pos = kv4_index(*positions, cache, at::kLong, "positions");
+    TORCH_CHECK(pos.dim() == 1 && pos.size(0) == tokens, "WOQ: positions must have one entry per token");
+    rot = table.size(1);
+    TORCH_CHECK(rot >= 16 && rot <= key.size(2), "WOQ: cos_sin has ", rot, " columns, heads ", key.size(2), " elements");
+  }
+  auto stream = at::cuda::getCurrentCUDAStream(cache.get_device());
+  WOQ_CHECK(woq_b200_kv4_append(&d, cache.data_ptr(), has_q ? q.data_ptr() : nullptr, has_q ? q.stride(0) : 0,
+                                has_q ? q.stride(1) : 0, has_q ? static_cast<int32_t>(q.size(1)) : 0, k.data_ptr(),
+                                k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), s.data_ptr<int64_t>(),
+                                turns ? pos.data_ptr<int64_t>() : nullptr, turns ? table.data_ptr<float>() : nullptr,
+                                turns ? table.size(0) : 0, static_cast<int32_t>(rot), interleaved, tokens,
+                                q_out.data_ptr(), stream.stream()));
+  return q_out;
+}
+
+std::tuple<at::Tensor, at::Tensor> kv4_cache_read(const at::Tensor& cache, const at::Tensor& slots, int64_t head_dim,
+                                                  at::ScalarType dtype) {
+  const woq_b200_kv4_desc d = kv4_desc(cache, head_dim, dtype);
+  c10::cuda::CUDAGuard guard(cache.device());
+  const at::Tensor s = kv4_index(slots, cache, at::kLong, "slots");
+  TORCH_CHECK(s.dim() == 1, "WOQ: slots must be one-dimensional");
+  at::Tensor k = at::empty({s.size(0), d.kv_heads, head_dim}, cache.options().dtype(dtype)), v = at::empty_like(k);
+  WOQ_CHECK(woq_b200_kv4_read(&d, cache.data_ptr(), s.data_ptr<int64_t>(), s.size(0), k.data_ptr(), v.data_ptr(),
+                              at::cuda::getCurrentCUDAStream(cache.get_device()).stream()));
+  return std::make_tuple(k, v);
+}
+
+at::Tensor kv4_cache_attention(const at::Tensor& query, const at::Tensor& cache, const at::Tensor& block_table,
+                               const at::Tensor& seq_lens, const c10::optional<at::Tensor>& query_starts,
+                               c10::optional<double> scale, bool causal) {
+  TORCH_CHECK(query.dim() == 3, "WOQ: query must be [rows, q heads, head_dim]");
+  const woq_b200_kv4_desc d = kv4_desc(cache, query.size(2), query.scalar_type());
+  c10::cuda::CUDAGuard guard(cache.device());
+  const at::Tensor q = kv4_rows(query, cache, query.scalar_type(), "query");
+  at::Tensor table = kv4_index(block_table, cache, at::kInt, "block_table");
+  const at::Tensor lens = kv4_index(seq_lens, cache, at::kInt, "seq_lens");
+  TORCH_CHECK(lens.dim() == 1 && table.dim() == 2 && table.size(0) == lens.size(0),
+              "WOQ: seq_lens must be [sequences] and block_table [sequences, pages]");
+  const int64_t batch = lens.size(0), tokens = q.size(0), heads = q.size(1);
+  TORCH_CHECK(heads >= 1 && heads <= INT32_MAX, "WOQ: the number of query heads is out of range");
+  at::Tensor starts;
+  if (query_starts.has_value() && query_starts->defined()) {
+    starts = kv4_index(*query_starts, cache, at::kInt, "query_starts");
+    TORCH_CHECK(starts.dim() == 1 && starts.size(0) == batch + 1, "WOQ: query_starts must be [sequences + 1]");
+  } else {
+    TORCH_CHECK(batch == tokens, "WOQ: without query_starts every sequence has one query row: got ", tokens, " rows for ",
+                batch, " sequences");
+  }
+  // (rows that belong to no sequence are zeros)
+  at::Tensor out = starts.defined() ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());
+  if (batch == 0 || tokens == 0) return out;
+  auto stream = at::cuda::getCurrentCUDAStream(cache.get_device());
+  const size_t need = woq_b200_kv4_attention_workspace_bytes(&d, batch, tokens, static_cast<int32_t>(heads));
+  TORCH_CHECK(need > 0, "WOQ: ", heads, " query heads over ", d.kv_heads, " cached ones of ", d.head_dim, " elements");
+  const Workspace ws = workspace_for(cache.get_device(), stream.stream(), need, out);
+  WOQ_CHECK(woq_b200_kv4_attention(&d, cache.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), static_cast<int32_t>(heads),
+                                   table.data_ptr<int32_t>(), table.stride(0), table.size(1), lens.data_ptr<int32_t>(),
+                                   starts.defined() ? starts.data_ptr<int32_t>() : nullptr, batch, tokens,
+                                   static_cast<float>(scale.value_or(1.0 / std::sqrt(static_cast<double>(d.head_dim)))), causal,
+                                   out.data_ptr(), out.stride(0), out.stride(1), ws.ptr, ws.bytes, stream.stream()));
+  return out;
+}
+
 // The linear on activations quantised by woq_rmsnorm_quant; `fusion` as in the C ABI (0 none,
 // 0x100 silu*mul on a gate/up context, ...), `others` the extra operands of the binary post-ops.
 at::Tensor woq_linear_prequant(const at::Tensor& qa, const at::Tensor& sa, const at::Tensor& zpa,
@@ -961,6 +1126,13 @@ TORCH_LIBRARY(torch_ipex, m) {
         "__torch__.torch.classes.ipex_prepack.WoqLinearOpContext[] down_ctx, "
         "Tensor routing_weights, bool is_distributed) -> Tensor");
   m.def("woq_rmsnorm_quant(Tensor input, Tensor weight, float eps, int act_quant_mode) -> (Tensor, Tensor, Tensor)");
+  m.def("woq_add_rmsnorm_quant(Tensor input, Tensor residual, Tensor weight, float eps, int act_quant_mode) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
+  m.def("kv4_cache_append(Tensor(a!) cache, Tensor key, Tensor value, Tensor slots, Tensor? query=None, "
+        "Tensor? positions=None, Tensor? cos_sin=None, bool interleaved=False) -> Tensor");
+  m.def("kv4_cache_read(Tensor cache, Tensor slots, int head_dim, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("kv4_cache_attention(Tensor query, Tensor cache, Tensor block_table, Tensor seq_lens, Tensor? query_starts=None, "
+        "float? scale=None, bool causal=True) -> Tensor");
   m.def("woq_linear_prequant(Tensor qa, Tensor sa, Tensor zpa, Tensor W_prepack, int fusion, Tensor[] others) -> Tensor");
   m.def("woq_check_status() -> ()", woq_check_status);
   m.def("woq_linear(Tensor input, Tensor qweight, str weight_dtype, int[] weight_shape, Tensor[] weight_scales, "
@@ -982,6 +1154,10 @@ TORCH_LIBRARY_IMPL(torch_ipex, CUDA, m) {
   m.impl("mixtral_moe_woq", mixtral_moe_woq);
   m.impl("deepseek_moe_woq", deepseek_moe_woq);
   m.impl("woq_rmsnorm_quant", woq_rmsnorm_quant);
+  m.impl("woq_add_rmsnorm_quant", woq_add_rmsnorm_quant);
+  m.impl("kv4_cache_append", kv4_cache_append);
+  m.impl("kv4_cache_read", kv4_cache_read);
+  m.impl("kv4_cache_attention", kv4_cache_attention);
   m.impl("woq_linear_prequant", woq_linear_prequant);
 }
 

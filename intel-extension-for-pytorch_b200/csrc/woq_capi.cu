@@ -1605,6 +1605,34 @@ int woq_b200_rmsnorm_quant(const void* x, int64_t ldx, const void* gamma, float 
   return WOQ_B200_OK;
 }
 
+int woq_b200_add_rmsnorm_quant(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* gamma, float eps,
+                               int64_t m, int64_t k, int32_t act_quant_mode, void* sum, int64_t lds, void* qa, void* sa,
+                               void* zpa, void* stream_) {
+  if (m == 0) return WOQ_B200_OK;
+  if (!x || !r || !gamma || !sum || !qa || !sa)
+    return fail(WOQ_B200_ERR_INVALID_ARG, "x, r, gamma, sum, qa and sa must be non-null");
+  if (m < 0 || m > INT32_MAX / 8 || k <= 0 || (k % 16) != 0)
+    return fail(WOQ_B200_ERR_INVALID_ARG, "woq_b200_add_rmsnorm_quant needs M >= 0 and K a positive multiple of 16");
+  if (k > woq::kAddNormMaxK)
+    return fail(WOQ_B200_ERR_UNSUPPORTED, "woq_b200_add_rmsnorm_quant takes rows of up to %d elements", woq::kAddNormMaxK);
+  if (act_quant_mode != WOQ_B200_ACT_PER_M && act_quant_mode != WOQ_B200_ACT_PER_M_SYM)
+    return fail(WOQ_B200_ERR_UNSUPPORTED,
+                "woq_b200_add_rmsnorm_quant quantises per token (WOQ_B200_ACT_PER_M or _PER_M_SYM), got mode %d",
+                act_quant_mode);
+  const int asym = act_quant_mode == WOQ_B200_ACT_PER_M;
+  if (asym && !zpa) return fail(WOQ_B200_ERR_INVALID_ARG, "the asymmetric mode writes zero points: zpa is null");
+  if (ldx < k || ldr < k || lds < k || ((ldx | ldr | lds) % 8) != 0 || !aligned16(x) || !aligned16(r) || !aligned16(gamma) ||
+      !aligned16(sum) || !aligned16(qa))
+    return fail(WOQ_B200_ERR_INVALID_ARG,
+                "x, r, gamma, sum and qa must be 16-byte aligned, row strides >= K and multiples of 8");
+  CUDA_TRY(woq::launch_add_rmsnorm_quant(static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(r), ldr,
+                                         static_cast<const __nv_bfloat16*>(gamma), eps, m, (int)k, asym,
+                                         static_cast<__nv_bfloat16*>(sum), lds, static_cast<int8_t*>(qa),
+                                         static_cast<float*>(sa), static_cast<int32_t*>(zpa),
+                                         static_cast<cudaStream_t>(stream_)));
+  return WOQ_B200_OK;
+}
+
 int woq_b200_linear_prequant(const woq_b200_ctx* c, const void* qa, const void* sa, const void* zpa, int64_t m,
                              int32_t fusion, const void* const* others, int32_t n_others, void* y, int64_t ldy,
                              void* workspace, size_t workspace_bytes, void* stream_) {
@@ -2073,6 +2101,8 @@ int woq_b200_workspace_status(void* workspace, void* stream_) {
   if (h != 0) {
     // a kernel that gave up may have left arrival counters behind: the whole header starts over
     CUDA_TRY(cudaMemsetAsync(workspace, 0, kWsHeaderBytes, stream));
+    if (h == woq::kStatusBadPage)
+      return fail(WOQ_B200_ERR_INVALID_ARG, "a block table named a page that the cache does not have: its keys were left out");
     return fail(WOQ_B200_ERR_DEVICE_WAIT, "a bounded in-kernel wait gave up (code %d)", h);
   }
   return WOQ_B200_OK;

@@ -357,6 +357,139 @@ __global__ void __launch_bounds__(256) rmsnorm_quant_kernel(const __nv_bfloat16*
   }
 }
 
+// The residual's addition, RMSNorm and the per-token quantiser: h = bf16(x + r), then what rmsnorm_quant_kernel does
+// on h.  A row is read once and stays in registers (PIECES of eight elements a thread, as bf16) from the sum to the
+// codes; CL CTAs of a cluster share a row and exchange their sums of squares and ranges through distributed shared
+// memory.
+__device__ __forceinline__ uint32_t add_bf16x2_rn(uint32_t a, uint32_t b) {
+  const float lo = __uint_as_float(a << 16) + __uint_as_float(b << 16);
+  const float hi = __uint_as_float(a & 0xffff0000u) + __uint_as_float(b & 0xffff0000u);
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <bool ASYM, int CL, int PIECES>
+__global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloat16* x, int64_t ldx,
+                                                                const __nv_bfloat16* r, int64_t ldr,
+                                                                const __nv_bfloat16* gamma, float eps, int k,
+                                                                __nv_bfloat16* sum, int64_t lds, int8_t* qa, float* sa,
+                                                                int32_t* zpa) {
+  __shared__ float red[16], mine[3];
+  const int64_t m = blockIdx.x / CL;
+  const int slice = blockIdx.x % CL, tid = threadIdx.x;
+  const int per = (k / 8 + CL - 1) / CL, p0 = slice * per, p1 = min(k / 8, p0 + per);  // pieces of this CTA
+  const uint4* gr = reinterpret_cast<const uint4*>(gamma);
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const uint4* xr = reinterpret_cast<const uint4*>(x + m * ldx);
+  const uint4* rr = reinterpret_cast<const uint4*>(r + m * ldr);
+  uint4* hr = reinterpret_cast<uint4*>(sum + m * lds);
+  uint32_t h[PIECES][4];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int at = p0 + tid + i * 256;
+    if (at < p1) {
+      const uint4 a = xr[at], b = rr[at];
+      h[i][0] = add_bf16x2_rn(a.x, b.x);
+      h[i][1] = add_bf16x2_rn(a.y, b.y);
+      h[i][2] = add_bf16x2_rn(a.z, b.z);
+      h[i][3] = add_bf16x2_rn(a.w, b.w);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int at = p0 + tid + i * 256;
+    if (at >= p1) break;
+    hr[at] = make_uint4(h[i][0], h[i][1], h[i][2], h[i][3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = __uint_as_float(h[i][j] << 16), b = __uint_as_float(h[i][j] & 0xffff0000u);
+      ss = fmaf(a, a, ss);
+      ss = fmaf(b, b, ss);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if ((tid & 31) == 0) red[tid >> 5] = ss;
+  __syncthreads();
+  ss = red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) ss += red[i];
+  if (CL > 1) {
+    if (tid == 0) mine[0] = ss;
+    cluster_sync_all();
+    ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < CL; ++c) ss += cluster_ld(&mine[0], c);
+  }
+  __syncthreads();
+  const float inv = __frsqrt_rn(__fdiv_rn(ss, static_cast<float>(k)) + eps);
+  float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int at = p0 + tid + i * 256;
+    if (at >= p1) break;
+    const uint4 g = gr[at];
+    const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(h[i][j] << 16) * inv * __uint_as_float(gw[j] << 16),
+                                                     __uint_as_float(h[i][j] & 0xffff0000u) * inv *
+                                                         __uint_as_float(gw[j] & 0xffff0000u));
+      h[i][j] = *reinterpret_cast<const uint32_t*>(&y);
+      const float a = __uint_as_float(h[i][j] << 16), b = __uint_as_float(h[i][j] & 0xffff0000u);
+      lo = fminf(lo, fminf(a, b));
+      hi = fmaxf(hi, fmaxf(a, b));
+    }
+  }
+  block_min_max(lo, hi, red);
+  if (CL > 1) {
+    if (tid == 0) {
+      mine[1] = lo;
+      mine[2] = hi;
+    }
+    cluster_sync_all();
+#pragma unroll
+    for (int c = 0; c < CL; ++c) {
+      lo = fminf(lo, cluster_ld(&mine[1], c));
+      hi = fmaxf(hi, cluster_ld(&mine[2], c));
+    }
+    cluster_sync_all();  // nobody leaves while another CTA may still read its range
+  }
+  float scale, zp = 0.f;
+  if (ASYM) {
+    scale = __fdiv_rn(hi - lo, 255.0f);
+    zp = -rintf(__fdiv_rn(lo, scale));
+    if (tid == 0 && slice == 0) zpa[m] = scale > 0.f ? static_cast<int32_t>(zp) : 0;
+  } else {
+    scale = __fdiv_rn(fmaxf(fabsf(hi), fabsf(lo)), 127.0f);
+  }
+  if (!(ss < INFINITY)) scale = __int_as_float(0x7fc00000);  // codes cannot say it: the row's scale does
+  if (tid == 0 && slice == 0) sa[m] = scale;
+  const float q_lo = ASYM ? 0.f : -128.f, q_hi = ASYM ? 255.f : 127.f;
+  uint2* qr = reinterpret_cast<uint2*>(qa + m * k);
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int at = p0 + tid + i * 256;
+    if (at >= p1) break;
+    uint32_t out[2] = {0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = __uint_as_float(h[i][j] << 16), b = __uint_as_float(h[i][j] & 0xffff0000u);
+      float ql = 0.f, qh = 0.f;
+      if (scale > 0.f) {
+        ql = fminf(fmaxf(rintf(__fdiv_rn(a, scale) + zp), q_lo), q_hi);
+        qh = fminf(fmaxf(rintf(__fdiv_rn(b, scale) + zp), q_lo), q_hi);
+      }
+      const uint32_t c = (static_cast<uint32_t>(static_cast<int>(ql)) & 0xffu) |
+                         ((static_cast<uint32_t>(static_cast<int>(qh)) & 0xffu) << 8);
+      out[j >> 1] |= c << ((j & 1) * 16);
+    }
+    qr[at] = make_uint2(out[0], out[1]);
+  }
+}
+
 // compensation[n] = sum over k of the weight codes of row n (plain [n][k] int8): what an
 // activation zero point contributes to every accumulator of that row.  One warp per row.
 __global__ void __launch_bounds__(256) weight_row_sum_kernel(const int8_t* w, int n, int k, int32_t* comp) {
@@ -463,6 +596,50 @@ cudaError_t launch_rmsnorm_quant(const __nv_bfloat16* x, int64_t ldx, const __nv
     rmsnorm_quant_kernel<false><<<m, 256, 0, stream>>>(x, ldx, gamma, eps, k, y, ldy, qa, sa, zpa);
   count_launch();
   return cudaGetLastError();
+}
+
+template <bool ASYM, int CL, int PIECES>
+static cudaError_t launch_add_norm(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* r, int64_t ldr,
+                                   const __nv_bfloat16* gamma, float eps, int64_t m, int k, __nv_bfloat16* sum,
+                                   int64_t lds, int8_t* qa, float* sa, int32_t* zpa, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(m * CL));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (CL > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = CL;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (dependent_launch_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, add_rmsnorm_quant_kernel<ASYM, CL, PIECES>, x, ldx, r, ldr, gamma, eps, k, sum, lds, qa,
+                            sa, zpa);
+}
+
+cudaError_t launch_add_rmsnorm_quant(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* r, int64_t ldr,
+                                     const __nv_bfloat16* gamma, float eps, int64_t m, int k, int asym,
+                                     __nv_bfloat16* sum, int64_t lds, int8_t* qa, float* sa, int32_t* zpa,
+                                     cudaStream_t stream) {
+  constexpr int kPer = 8 * 256;  // elements that one CTA holds per piece
+#define ADD_NORM(CL, PIECES)                                                                                             \
+  return asym ? launch_add_norm<true, CL, PIECES>(x, ldx, r, ldr, gamma, eps, m, k, sum, lds, qa, sa, zpa, stream)       \
+              : launch_add_norm<false, CL, PIECES>(x, ldx, r, ldr, gamma, eps, m, k, sum, lds, qa, sa, zpa, stream)
+  if (k <= kPer) ADD_NORM(1, 1);
+  if (m <= 128 && k <= 4 * kPer) ADD_NORM(4, 1);  // few rows: four CTAs each
+  if (k <= 2 * kPer) ADD_NORM(1, 2);
+  if (k <= 4 * kPer) ADD_NORM(1, 4);
+  if (k <= 8 * kPer) ADD_NORM(1, 8);
+  ADD_NORM(8, 8);
+#undef ADD_NORM
 }
 
 cudaError_t launch_weight_row_sum(const int8_t* plain, int n, int k, int32_t* comp, cudaStream_t stream) {

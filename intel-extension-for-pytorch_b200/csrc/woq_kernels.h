@@ -237,6 +237,11 @@ cudaError_t launch_quant_act(const __nv_bfloat16* x, int64_t ldx, int m, int k, 
 cudaError_t launch_rmsnorm_quant(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* gamma, float eps, int m,
                                  int k, int asym, __nv_bfloat16* y, int64_t ldy, int8_t* qa, float* sa, int32_t* zpa,
                                  cudaStream_t stream);
+cudaError_t launch_add_rmsnorm_quant(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* r, int64_t ldr,
+                                     const __nv_bfloat16* gamma, float eps, int64_t m, int k, int asym,
+                                     __nv_bfloat16* sum, int64_t lds, int8_t* qa, float* sa, int32_t* zpa,
+                                     cudaStream_t stream);
+constexpr int kAddNormMaxK = 8 * 8 * 8 * 256;  // a cluster of eight CTAs holds a row in registers
 cudaError_t launch_weight_row_sum(const int8_t* plain, int n, int k, int32_t* comp, cudaStream_t stream);
 
 // ---- INT8 compute with K-block scaling (woq_int8_block.cu) --------------------------------
@@ -382,6 +387,49 @@ __host__ __device__ inline int tile_row_to_n(int n_total, int gate_up, int tile,
   if (gate_up) return row < 32 ? tile * 32 + row : n_total / 2 + tile * 32 + (row - 32);
   return tile * kTileN + row;
 }
+
+// ---- paged 4-bit key/value cache (woq_kv4*.cu; layout: woq_kv4_common.cuh) ------------------------------------
+struct Kv4AppendParams {
+  const uint16_t* q;  // [tokens][q_heads][D], strides in elements; or null with q_heads 0
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* q_out;    // [tokens][q_heads][D]
+  uint8_t* cache;
+  const int64_t* slots;      // [tokens]
+  const int64_t* positions;  // [tokens], or null with rot 0
+  const float* cos_sin;      // [max_pos][rot]: cosines, then sines
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, max_pos, num_slots;
+  int q_heads, kv_heads, page_blocks, rot, interleaved;
+};
+cudaError_t launch_kv4_append(const Kv4AppendParams& p, int f16, int d, int g, int64_t tokens, cudaStream_t stream);
+struct Kv4ReadParams {
+  const uint8_t* cache;
+  const int64_t* slots;
+  uint16_t* k;  // [tokens][kv_heads][D]
+  uint16_t* v;
+  int64_t tokens, num_slots;
+  int kv_heads, page_blocks;
+};
+cudaError_t launch_kv4_read(const Kv4ReadParams& p, int f16, int d, int g, cudaStream_t stream);
+struct Kv4AttendParams {
+  const uint16_t* q;  // [tokens][q_heads][D], strides in elements
+  uint16_t* out;      // the same
+  const uint8_t* cache;
+  const int32_t* table;   // [batch][max_pages] page numbers, rows `table_ld` apart
+  const int32_t* lens;    // [batch] cached tokens
+  const int32_t* starts;  // [batch + 1] first row of every sequence in q, or null: one row each
+  float* partials;        // [CTAs][2][rows of a tile * (D + 2)]
+  uint32_t* counters;     // [CTAs], zero between calls
+  int* status;
+  int64_t q_tok, q_head, o_tok, o_head, table_ld, num_pages;
+  float scale;            // of the scores, times log2 e
+  int batch, tokens, q_heads, kv_heads, heads;  // heads: query heads of a kv head
+  int page_blocks, max_blocks, causal;
+};
+int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d);
+size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int d, int num_sms);
+cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, int num_sms, cudaStream_t stream);
+constexpr int kStatusBadPage = 901;  // a block table names a page that the cache does not have
 
 void count_launch();
 

@@ -60,6 +60,12 @@ EXPORTS = [
     "woq_b200_dump_dequant",
     "woq_b200_int8_internals",
     "woq_b200_rmsnorm_quant",
+    "woq_b200_add_rmsnorm_quant",
+    "woq_b200_kv4_bytes",
+    "woq_b200_kv4_append",
+    "woq_b200_kv4_read",
+    "woq_b200_kv4_attention_workspace_bytes",
+    "woq_b200_kv4_attention",
     "woq_b200_linear_prequant",
     "woq_b200_int8_block_internals",
     "woq_b200_int8_block_size",
@@ -94,6 +100,19 @@ class Desc(ctypes.Structure):
         ("bias_dtype", ctypes.c_int32),
         ("layout_flags", ctypes.c_int32),
         ("kernel_hint", ctypes.c_int32),
+    ]
+
+
+class Kv4Desc(ctypes.Structure):
+    """woq_b200_kv4_desc: a paged 4-bit key/value cache."""
+
+    _fields_ = [
+        ("num_pages", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("group_size", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
     ]
 
 
@@ -148,6 +167,17 @@ def lib() -> ctypes.CDLL:
     L.woq_b200_dump_dequant.argtypes = [vp, vp, vp]
     L.woq_b200_int8_internals.argtypes = [vp, vp, i64, i64, vp, vp, vp, vp, sz, vp]
     L.woq_b200_rmsnorm_quant.argtypes = [vp, i64, vp, ctypes.c_float, i64, i64, i32, vp, i64, vp, vp, vp, vp]
+    L.woq_b200_add_rmsnorm_quant.argtypes = [vp, i64, vp, i64, vp, ctypes.c_float, i64, i64, i32, vp, i64, vp, vp, vp, vp]
+    kv4 = ctypes.POINTER(Kv4Desc)
+    L.woq_b200_kv4_bytes.argtypes = [kv4]
+    L.woq_b200_kv4_bytes.restype = sz
+    L.woq_b200_kv4_append.argtypes = [kv4, vp, vp, i64, i64, i32, vp, i64, i64, vp, i64, i64, vp, vp, vp, i64, i32, i32,
+                                      i64, vp, vp]
+    L.woq_b200_kv4_read.argtypes = [kv4, vp, vp, i64, vp, vp, vp]
+    L.woq_b200_kv4_attention_workspace_bytes.argtypes = [kv4, i64, i64, i32]
+    L.woq_b200_kv4_attention_workspace_bytes.restype = sz
+    L.woq_b200_kv4_attention.argtypes = [kv4, vp, vp, i64, i64, i32, vp, i64, i64, vp, vp, i64, i64, ctypes.c_float, i32,
+                                         vp, i64, i64, vp, sz, vp]
     L.woq_b200_linear_prequant.argtypes = [vp, vp, vp, vp, i64, i32, ctypes.POINTER(vp), i32, vp, i64, vp, sz, vp]
     L.woq_b200_int8_block_internals.argtypes = [vp, vp, i64, i64, vp, vp, vp, vp, vp, sz, vp]
     L.woq_b200_int8_block_size.argtypes = [vp]

@@ -17,7 +17,9 @@ class _IPEXRmsNormQuantLinears(nn.Module):
     """norm: a module with `weight` [K] and `eps` / `variance_epsilon` (nn.RMSNorm, LlamaRMSNorm).
     linears: WeightOnlyQuantizedLinear modules with INT8 weights, WoqLowpMode.INT8 and a per-token
     activation mode, all the same mode (_IPEXlinearFusedGateUp modules are accepted too: they
-    apply silu * mul).  forward(x) returns the tuple of their outputs on rmsnorm(x)."""
+    apply silu * mul).  forward(x) returns the tuple of their outputs on rmsnorm(x);
+    forward(x, residual) adds the residual first, in the same kernel, and returns (the tuple, the sum): behind
+    layers whose output cannot add it in an epilogue (a mixture of experts, an all-reduce)."""
 
     def __init__(self, norm, linears):
         super().__init__()
@@ -32,11 +34,15 @@ class _IPEXRmsNormQuantLinears(nn.Module):
         for m in linears:
             assert int(getattr(m, "_lowp_mode", -1)) == 3, "the fused quantiser feeds INT8-compute linears"
 
-    def forward(self, x):
-        qa, sa, zpa = torch.ops.torch_ipex.woq_rmsnorm_quant(x, self.weight, self.eps, self.act_quant_mode)
+    def forward(self, x, residual=None):
+        if residual is None:
+            qa, sa, zpa = torch.ops.torch_ipex.woq_rmsnorm_quant(x, self.weight, self.eps, self.act_quant_mode)
+        else:
+            total, qa, sa, zpa = torch.ops.torch_ipex.woq_add_rmsnorm_quant(x, residual, self.weight, self.eps,
+                                                                            self.act_quant_mode)
         outs = []
         for m in self.linears:
             fusion = FUSE_SILU_MUL if getattr(m, "is_gate_up", False) else FUSE_NONE
             outs.append(torch.ops.torch_ipex.woq_linear_prequant(qa, sa, zpa, m._op_context.get_data_handle(),
                                                                  fusion, []))
-        return tuple(outs)
+        return tuple(outs) if residual is None else (tuple(outs), total)
