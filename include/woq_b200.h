@@ -441,7 +441,8 @@ size_t woq_b200_kv4_bytes(const woq_b200_kv4_desc* desc);
  * Rotated keys are rounded to `dtype` before they are quantised.  q may be null with q_heads 0.
  * A slot outside the cache (-1 for padding) stores nothing; a position outside the table stores nothing either and
  * makes the token's q_out NaN.  The slots of one call must be distinct.  Where a head's key or value has an element
- * that is not finite, the key reads back as NaN (and scores NaN) and a value with such an element as zeros. */
+ * that is not finite (bf16: not below 2^61 in magnitude), the key reads back as NaN (and scores NaN) and a value with
+ * such an element as zeros. */
 int woq_b200_kv4_append(const woq_b200_kv4_desc* desc, void* cache, const void* q, int64_t q_token_stride,
                         int64_t q_head_stride, int32_t q_heads, const void* k, int64_t k_token_stride,
                         int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
@@ -457,7 +458,7 @@ int woq_b200_kv4_read(const woq_b200_kv4_desc* desc, const void* cache, const in
  * rows query_starts[b] .. query_starts[b + 1] - 1 (device array of batch + 1 entries; null: row b alone, and
  * tokens == batch).  `causal`: its queries are its last tokens, and a query does not see the tokens after it.
  * q_heads is a multiple of kv_heads; query head h reads kv head h / (q_heads / kv_heads).  A row that sees nothing is
- * zeros; rows of `out` that belong to no sequence stay as they are.  Lengths, tables and starts are read on the
+ * zeros (scales are below 1e18; bf16 keys and values below 2^-62 lose digits); rows of `out` that belong to no sequence stay as they are.  Lengths, tables and starts are read on the
  * device: a captured call follows them.  Workspace as for woq_b200_linear (its header zero before the first use).
  * Keys of pages that the cache does not have are left out, and woq_b200_workspace_status then returns
  * WOQ_B200_ERR_INVALID_ARG.  Two calls with the same arguments give the same bits. */

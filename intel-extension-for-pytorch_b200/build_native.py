@@ -35,6 +35,7 @@ CUDA_SOURCES = [
     "woq_i8_pair.cu",
     "woq_kv4.cu",
     "woq_kv4_attend.cu",
+    "woq_kv4_prompt.cu",
     "woq_kv4_capi.cu",
 ]
 NVCC_FLAGS = [

@@ -422,13 +422,15 @@ struct Kv4AttendParams {
   uint32_t* counters;     // [CTAs], zero between calls
   int* status;
   int64_t q_tok, q_head, o_tok, o_head, table_ld, num_pages;
-  float scale;            // of the scores, times log2 e
+  float scale;            // of the scores, times log2 e (below 2^63)
   int batch, tokens, q_heads, kv_heads, heads;  // heads: query heads of a kv head
   int page_blocks, max_blocks, causal;
+  int page_shift;         // log2 of page_blocks, or -1 (set by the launch)
 };
 int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d);
 size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int d, int num_sms);
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, int num_sms, cudaStream_t stream);
+cudaError_t launch_kv4_prompt(const Kv4AttendParams& p, int f16, int d, int g, cudaStream_t stream);
 constexpr int kStatusBadPage = 901;  // a block table names a page that the cache does not have
 
 void count_launch();

@@ -38,7 +38,7 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&c)[8],
   for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) < INFINITY;
+    finite = finite && fabsf(x[i]) < T::kTooLarge;
   }
 #pragma unroll
   for (int o = 1; o < LG; o <<= 1) {
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendParams p) {
       float y[8];
       unpack8<T>(*reinterpret_cast<const uint4*>(p.v + token * p.v_tok + head * p.v_head + sub * 8), y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) finite = finite && fabsf(y[i]) < INFINITY;
+      for (int i = 0; i < 8; ++i) finite = finite && fabsf(y[i]) < T::kTooLarge;
     }
     const uint32_t bad = __ballot_sync(0xffffffffu, !finite);
     const uint32_t row_mask = kLanes == 32 ? 0xffffffffu : ((1u << (kLanes & 31)) - 1) << ((threadIdx.x & 31) / kLanes * kLanes);

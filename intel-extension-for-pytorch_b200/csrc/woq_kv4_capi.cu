@@ -158,7 +158,7 @@ int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const 
   if (!query_starts && batch != tokens)
     return set_error(WOQ_B200_ERR_INVALID_ARG, "without query_starts every sequence has one query row: %lld rows for %lld "
                      "sequences", (long long)tokens, (long long)batch);
-  if (!std::isfinite(scale)) return set_error(WOQ_B200_ERR_INVALID_ARG, "the scale must be finite");
+  if (!(std::fabs(scale) < 1e18f)) return set_error(WOQ_B200_ERR_INVALID_ARG, "the scale must be a number below 1e18");
   if (tokens == 0 || batch == 0) return WOQ_B200_OK;
   if (max_pages > 0 && (INT32_MAX - 15) / max_pages < d->page_size)
     return set_error(WOQ_B200_ERR_UNSUPPORTED, "a block table of %lld pages of %d tokens passes 2^31 tokens", (long long)max_pages,

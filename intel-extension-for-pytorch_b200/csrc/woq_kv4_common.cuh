@@ -46,7 +46,9 @@ __host__ __device__ constexpr int kv4_value_half(int d, int r, int half, int j, 
 // Arithmetic of the two 16-bit types
 struct Kv4Bf16 {
   using type = __nv_bfloat16;
+  static constexpr bool kIsBf16 = true;
   static constexpr uint32_t kMagic = 0x43004300u;  // 128 + c with the code in the low bits
+  static constexpr float kTooLarge = 2305843009213693952.f;  // 2^61: the attention kernel scales by 2^69
   static constexpr uint32_t kNan = 0x7fffu;
   static __device__ __forceinline__ float to_float(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
   static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
@@ -65,12 +67,18 @@ struct Kv4Bf16 {
     return r;
   }
   static __device__ __forceinline__ void mma(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-    mma_bf16_16816(d, a, b0, b1);
+    // (not volatile: independent products may move past one another)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 };
 struct Kv4Fp16 {
   using type = __half;
+  static constexpr bool kIsBf16 = false;
   static constexpr uint32_t kMagic = 0x64006400u;  // 1024 + c
+  static constexpr float kTooLarge = INFINITY;
   static constexpr uint32_t kNan = 0x7fffu;
   static __device__ __forceinline__ float to_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   static __device__ __forceinline__ float lo(uint32_t v) { return to_float(static_cast<uint16_t>(v & 0xffffu)); }
@@ -93,8 +101,7 @@ struct Kv4Fp16 {
     return r;
   }
   static __device__ __forceinline__ void mma(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
         "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));

@@ -1,0 +1,498 @@
+// Attention of prompts over the paged 4-bit cache (layout: woq_kv4_common.cuh) on the tensor cores (tcgen05):
+//   o = sum_j softmax_j(scale * q . k_j) v_j, causal from the last token backwards or over all keys.
+//
+// A CTA takes one kv head of one sequence and NQ tiles of 128 query rows (a row is a token's query head; the heads
+// of a kv head lie next to one another, so they share its keys), and walks over the keys in tiles of KT:
+//   warps 0 .. 4 NQ - 1   softmax: thread = query row.  Scores from tensor memory, probabilities back over them
+//   4 warps               keys:   codes of a tile to T in shared memory, K-major with 128-byte swizzle
+//   4 warps               values: the same, transposed (a row per element, its keys next to one another)
+//   1 warp                issues S = Q K^T and O += P V; allocates tensor memory
+// The products of one tile of rows run while the other tile's softmax does.  Codes are loaded straight into
+// registers, one tile ahead; the dequantised values (bf16: times 2^-64, see Dequant) never leave the SM.
+// The running reference of the maximum is raised only when a score passes it by 8 (log2): P is at most 256 and O is
+// rescaled seldom.
+#include "woq_kernels.h"
+#include "woq_kv4_common.cuh"
+#include "woq_kv4_dequant.cuh"
+#include "woq_tc_common.cuh"
+
+namespace woq {
+
+namespace {
+
+template <int D>
+struct Shape {
+  static constexpr int kNQ = D == 256 ? 1 : 2;    // tiles of 128 rows
+  static constexpr int kKeys = D == 256 ? 64 : 128;
+  static constexpr int kRows = 128 * kNQ;
+  static constexpr int kSoftmaxWarps = 4 * kNQ, kKeyWarp0 = kSoftmaxWarps, kValueWarp0 = kKeyWarp0 + 4, kMmaWarp = kValueWarp0 + 4;
+  static constexpr int kThreads = (kMmaWarp + 1) * 32;
+  static constexpr int kQBytes = 128 * D * 2, kKBytes = kKeys * D * 2;  // of a tile of queries, of keys or values
+  static constexpr int q = 1024, k = q + kNQ * kQBytes, v = k + 2 * kKBytes, total = v + 2 * kKBytes + 1024;
+};
+static_assert(Shape<64>::total <= 227 * 1024 && Shape<128>::total <= 227 * 1024 && Shape<256>::total <= 227 * 1024, "shared memory");
+
+struct Header {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint32_t tmem;
+  int abort_flag;
+  int b, tile;
+};
+static_assert(sizeof(Header) <= 1024, "header");
+
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      :
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// The sequence and tile of rows of a CTA (b = batch: none), found by one warp.  A sequence's last rows see most keys:
+// they go first.
+template <int ROWS>
+__device__ __forceinline__ void find_tile(const Kv4AttendParams& p, int64_t at, int& b_out, int& tile_out) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  b_out = p.batch;
+  tile_out = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    int64_t tiles = 0;
+    if (b0 + lane < p.batch) {
+      const int s0 = min(max(p.starts[b0 + lane], 0), p.tokens), s1 = min(max(p.starts[b0 + lane + 1], s0), p.tokens);
+      tiles = (static_cast<int64_t>(s1 - s0) * p.heads + ROWS - 1) / ROWS;
+    }
+    int64_t end = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end += x;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, before + end > at);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      b_out = b0 + src;
+      tile_out = static_cast<int>(__shfl_sync(0xffffffffu, before + end - 1 - at, src));
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, end, 31);
+  }
+}
+
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const __grid_constant__ Kv4AttendParams p) {
+  using S = Shape<D>;
+  constexpr int NQ = S::kNQ, KT = S::kKeys, kRows = S::kRows, kBlock = kv4_block_bytes(D, G), ng = D / G;
+  constexpr int W = kv4_width(D), nw = W / 32, kHalves = D / W, kGroups = ng / kHalves, kWordsPerGroup = G / 32;
+  constexpr uint32_t kFormat = T::kIsBf16 ? 1 : 0;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  Header* hd = reinterpret_cast<Header*>(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &hd->abort_flag;
+
+  if (warp == S::kMmaWarp) {
+    tmem_alloc(&hd->tmem, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&hd->k_full[i], 128);
+      mbar_init(&hd->k_empty[i], 1);
+      mbar_init(&hd->v_full[i], 128);
+      mbar_init(&hd->v_empty[i], 1);
+      mbar_init(&hd->s_full[i], 1);
+      mbar_init(&hd->p_full[i], 128);
+      mbar_init(&hd->o_full[i], 1);
+    }
+    mbar_fence_init();
+    hd->abort_flag = 0;
+  }
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int h = blockIdx.x % p.kv_heads;
+  if (warp == 0) {
+    int b, tile;
+    find_tile<kRows>(p, blockIdx.x / p.kv_heads, b, tile);
+    if (lane == 0) {
+      hd->b = b;
+      hd->tile = tile;
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = hd->tmem;
+  const int b = hd->b, tile = hd->tile;
+  if (b < p.batch) {
+    const int q0 = min(max(p.starts[b], 0), p.tokens), n_tok = min(max(p.starts[b + 1], q0), p.tokens) - q0;
+    const int len = min(max(p.lens[b], 0), p.max_blocks * kKv4Tokens);
+    const int rows = n_tok * p.heads;                 // of the sequence
+    const int row_base = tile * kRows;
+    int tiles_of[NQ], n_max = 0;                      // tiles of keys that a tile of rows sees
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      const int last = min(rows, row_base + (i + 1) * 128) - 1;
+      int limit = p.causal ? len - n_tok + last / p.heads + 1 : len;
+      if (last < row_base + i * 128) limit = 0;       // no rows
+      tiles_of[i] = (max(0, min(limit, len)) + KT - 1) / KT;
+      n_max = max(n_max, tiles_of[i]);
+    }
+    const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_ld;
+    // the block that holds key `key` < len of this head; null: its page does not exist
+    auto block_of = [&](int key) -> const uint8_t* {
+      const int blk = key / kKv4Tokens, page_at = p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks;
+      const int page = table[page_at], inner = blk - page_at * p.page_blocks;
+      if (page < 0 || page >= p.num_pages) return nullptr;
+      return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + h) * p.page_blocks + inner) * kBlock;
+    };
+
+    // ---- queries: K-major, 64 elements a 128-byte row, 16-byte chunks swizzled ----
+    for (int i = threadIdx.x; i < kRows * (D / 8); i += S::kThreads) {
+      const int row = i / (D / 8), ch = i % (D / 8), at = row_base + row;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (at < rows)
+        x = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(q0 + at / p.heads) * p.q_tok +
+                                            static_cast<int64_t>(h * p.heads + at % p.heads) * p.q_head + ch * 8);
+      if (p.scale < 0.f) {  // the sign of the scale, so that the largest product is the largest score
+        x.x ^= 0x80008000u;
+        x.y ^= 0x80008000u;
+        x.z ^= 0x80008000u;
+        x.w ^= 0x80008000u;
+      }
+      const int r = row & 127;
+      *reinterpret_cast<uint4*>(smem + S::q + (row >> 7) * S::kQBytes + (ch >> 3) * (128 * 128) + r * 128 +
+                                (((ch & 7) ^ (r & 7)) << 4)) = x;
+    }
+    fence_async_proxy();
+    __syncthreads();
+
+    if (warp < S::kSoftmaxWarps) {
+      // ==== softmax ====
+      const int i = warp >> 2, quarter = warp & 3, row = row_base + i * 128 + quarter * 32 + lane;
+      const uint32_t t_s = tmem + i * 256 + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 128;
+      const int n = NQ == 1 || i == 0 ? tiles_of[0] : tiles_of[NQ - 1];
+      int sees = p.causal ? len - n_tok + row / p.heads + 1 : len;
+      if (row >= rows) sees = len;  // (a row of zeros that nobody reads)
+      sees = min(sees, len);
+      int all_see = sees;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, o));
+      const float scale = fabsf(p.scale);
+      float top = -INFINITY, sum = 0.f;
+      for (int j = 0; j < n; ++j) {
+        const int key0 = j * KT;
+        uint32_t gone = 0;  // blocks of the tile whose page does not exist
+        if (key0 + lane * kKv4Tokens < len && lane < KT / kKv4Tokens) gone = block_of(key0 + lane * kKv4Tokens) == nullptr;
+        gone = __ballot_sync(0xffffffffu, gone);
+        const bool masked = key0 + KT > all_see || gone;
+        if (gone && lane == 0) atomicCAS(p.status, 0, kStatusBadPage);
+        mbar_wait(&hd->s_full[i], j & 1, abort_flag, p.status, 920);
+        tc_fence_after_sync();
+        float most = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld_x32(t_s + c * 32, r);
+          tc_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (key0 + c * 32 + e >= sees || ((gone >> (c * 2 + e / 16)) & 1)) r[e] = 0xff800000u;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) most = fmaxf(most, __uint_as_float(r[e]));
+        }
+        most *= scale;  // (NaN for a row that sees nothing of the tile at a scale of 0: ignored)
+        if (__any_sync(0xffffffffu, most - top > 8.f)) {
+          const float m = fmaxf(most, top), f = top == m ? 1.f : exp2f(top - m);
+          top = m;
+          sum *= f;
+          if (j > 0) {
+            mbar_wait(&hd->o_full[i], (j - 1) & 1, abort_flag, p.status, 921);
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t r[32];
+              tmem_ld_x32(t_o + c * 32, r);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+              tmem_st_x32(t_o + c * 32, r);
+            }
+          }
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) {
+          uint32_t r[32], out[16];
+          tmem_ld_x32(t_s + c * 32, r);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float x = fmaf(__uint_as_float(r[e]), scale, -base), y = fmaf(__uint_as_float(r[e + 1]), scale, -base);
+            if (masked) {
+              const bool no = (gone >> (c * 2 + e / 16)) & 1;
+              if (no || key0 + c * 32 + e >= sees) x = -INFINITY;
+              if (no || key0 + c * 32 + e + 1 >= sees) y = -INFINITY;
+            }
+            x = exp2_approx(x);
+            y = exp2_approx(y);
+            sum += x + y;
+            out[e / 2] = T::pack(x, y);
+          }
+          tmem_st_x16(t_s + c * 16, out);
+        }
+        tc_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive(&hd->p_full[i]);
+      }
+      // ---- the rows' results ----
+      if (n > 0) {
+        mbar_wait(&hd->o_full[i], (n - 1) & 1, abort_flag, p.status, 922);
+        tc_fence_after_sync();
+      }
+      const float inv = sum == 0.f ? 0.f : Dequant<T>::kBack / sum;
+      const int token = row / p.heads;
+      uint16_t* dst = p.out + static_cast<int64_t>(q0 + token) * p.o_tok +
+                      static_cast<int64_t>(h * p.heads + row - token * p.heads) * p.o_head;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        if (n > 0) {
+          tmem_ld_x32(t_o + c * 32, r);
+          tc_wait_ld();
+        }
+        if (row < rows) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = n > 0 && sum != 0.f ? T::pack(__uint_as_float(r[e * 8 + k * 2]) * inv, __uint_as_float(r[e * 8 + k * 2 + 1]) * inv) : 0u;
+            *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      tc_fence_before_sync();
+    } else if (warp < S::kValueWarp0) {
+      // ==== keys: a thread has words [t][..] of four rows (and halves) of a tile ====
+      // lanes: 8 rows x 4 words, so that eight lanes of one t write eight rows' chunks to different banks
+      constexpr int kItems = KT * 4 * kHalves / 128;
+      const int kw = warp - S::kKeyWarp0;
+      uint32_t w[kItems][nw], par[kItems][kGroups];
+      auto row_of = [&](int it) { return (it / kHalves * 4 + kw) * 8 + (lane & 7); };
+      const int t = lane >> 3;
+      auto load = [&](int j) {
+#pragma unroll
+        for (int it = 0; it < kItems; ++it) {
+          const int key = j * KT + row_of(it), hh = it % kHalves;
+          const uint8_t* blk = key < len ? block_of(key) : nullptr;
+          const int r = key % kKv4Tokens;
+          if (blk) {
+            load_words(blk + r * (D / 2) + hh * 64 + t * nw * 4, w[it]);
+            load_words(blk + kv4_key_params(D) + (r * ng + hh * kGroups) * 4, par[it]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < nw; ++k) w[it][k] = 0;
+#pragma unroll
+            for (int k = 0; k < kGroups; ++k) par[it][k] = 0;
+          }
+        }
+      };
+      if (n_max > 0) load(0);
+      for (int j = 0; j < n_max; ++j) {
+        uint8_t* dst = smem + S::k + (j & 1) * S::kKBytes;
+        if (j >= 2) mbar_wait(&hd->k_empty[j & 1], ((j >> 1) - 1) & 1, abort_flag, p.status, 923);
+#pragma unroll
+        for (int it = 0; it < kItems; ++it) {
+          const int row = row_of(it), hh = it % kHalves;
+          Dequant<T> dq;
+#pragma unroll
+          for (int k = 0; k < nw; ++k) {
+            if (k % kWordsPerGroup == 0) dq.same(par[it][k / kWordsPerGroup]);
+            uint32_t x[4];
+            dq.values(w[it][k], x);
+            const int ch = hh * 16 + 4 * k + t;  // 8 elements from 8 ch
+            *reinterpret_cast<uint4*>(dst + (ch >> 3) * (KT * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
+                make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+        fence_async_proxy();
+        mbar_arrive(&hd->k_full[j & 1]);
+        if (j + 1 < n_max) load(j + 1);
+      }
+    } else if (warp < S::kMmaWarp) {
+      // ==== values: a thread has elements g + 8 n + 32 k (of a half) of eight tokens of a tile ====
+      const int id = (warp - S::kValueWarp0) * 4 + (lane >> 3), g = lane & 7;
+      const int hh = id % kHalves, eight = id / kHalves;  // half of the head, eight tokens
+      uint32_t w[4][nw], par[8][kGroups];
+      auto load = [&](int j) {
+        const int key = j * KT + eight * 8;
+        const uint8_t* blk = key < len ? block_of(key) : nullptr;
+        const int p0 = (eight & 1) * 4;  // first pair of tokens in its block
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (blk) {
+            load_words(blk + 8 * D + hh * W * 8 + (g * 8 + ((p0 + k) ^ kv4_swap(D, g))) * (nw * 4), w[k]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < nw; ++e) w[k][e] = 0;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (blk && key + k < len) {
+            load_words(blk + kv4_value_params(D, G) + ((p0 * 2 + k) * ng + hh * kGroups) * 4, par[k]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kGroups; ++e) par[k][e] = 0;  // tokens behind the last one hold anything
+          }
+        }
+      };
+      if (n_max > 0) load(0);
+      for (int j = 0; j < n_max; ++j) {
+        uint8_t* dst = smem + S::v + (j & 1) * S::kKBytes;
+        if (j >= 2) mbar_wait(&hd->v_empty[j & 1], ((j >> 1) - 1) & 1, abort_flag, p.status, 924);
+        Dequant<T> dq[4];
+#pragma unroll
+        for (int k = 0; k < nw; ++k) {
+          if (k % kWordsPerGroup == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dq[e].pair(par[2 * e][k / kWordsPerGroup], par[2 * e + 1][k / kWordsPerGroup]);
+          }
+          uint32_t x[4][4];  // [pair of tokens][n]
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dq[e].values(w[e][k], x[e]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int d = hh * 128 + 32 * k + 8 * n + g;
+            *reinterpret_cast<uint4*>(dst + (eight >> 3) * (D * 128) + d * 128 + (((eight & 7) ^ g) << 4)) =
+                make_uint4(x[0][n], x[1][n], x[2][n], x[3][n]);
+          }
+        }
+        fence_async_proxy();
+        mbar_arrive(&hd->v_full[j & 1]);
+        if (j + 1 < n_max) load(j + 1);
+      }
+    } else {
+      if (lane == 0) {
+      // ==== products ====
+      const uint32_t id_s = umma_idesc(KT, kFormat, kFormat, 1), id_o = umma_idesc(D, kFormat, kFormat, 1);
+      const uint32_t q_base = smem_u32(smem + S::q), k_base = smem_u32(smem + S::k), v_base = smem_u32(smem + S::v);
+      auto scores = [&](int i, int j) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          umma_f16_ss(tmem + i * 256, umma_desc_k128(q_base + i * S::kQBytes + (s >> 2) * (128 * 128) + (s & 3) * 32),
+                      umma_desc_k128(k_base + (j & 1) * S::kKBytes + (s >> 2) * (KT * 128) + (s & 3) * 32), id_s, s > 0);
+        tc_commit(&hd->s_full[i]);
+      };
+      if (n_max > 0) {
+        mbar_wait(&hd->k_full[0], 0, abort_flag, p.status, 925);
+        tc_fence_after_sync();
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          if (tiles_of[i] > 0) scores(i, 0);
+        tc_commit(&hd->k_empty[0]);
+      }
+      for (int j = 0; j < n_max; ++j) {
+        mbar_wait(&hd->v_full[j & 1], (j >> 1) & 1, abort_flag, p.status, 926);
+        if (j + 1 < n_max) mbar_wait(&hd->k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag, p.status, 927);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          if (j < tiles_of[i]) {
+            mbar_wait(&hd->p_full[i], j & 1, abort_flag, p.status, 928);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int s = 0; s < KT / 16; ++s)
+              umma_f16_ts(tmem + i * 256 + 128, tmem + i * 256 + s * 8,
+                          umma_desc_k128(v_base + (j & 1) * S::kKBytes + (s >> 2) * (D * 128) + (s & 3) * 32), id_o, j > 0 || s > 0);
+            tc_commit(&hd->o_full[i]);
+          }
+          if (j + 1 < tiles_of[i]) scores(i, j + 1);
+        }
+        tc_commit(&hd->v_empty[j & 1]);
+        if (j + 1 < n_max) tc_commit(&hd->k_empty[(j + 1) & 1]);
+      }
+      // the last commits of the barriers that nobody waits for end with the products before them
+      if (n_max > 0) mbar_wait(&hd->v_empty[(n_max - 1) & 1], ((n_max - 1) >> 1) & 1, abort_flag, p.status, 929);
+      tc_fence_before_sync();
+      }
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  if (warp == S::kMmaWarp) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <typename T, int D, int G>
+cudaError_t launch_one(const Kv4AttendParams& p, cudaStream_t stream) {
+  using S = Shape<D>;
+  auto kernel = kv4_prompt_kernel<T, D, G>;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total)) return e;
+  cudaLaunchConfig_t cfg = {};
+  const int64_t tiles = ceil_div(static_cast<int64_t>(p.tokens) * p.heads, S::kRows) + p.batch;
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.kv_heads));
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = S::total;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  if (dependent_launch_enabled()) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <typename T>
+cudaError_t launch_shape(const Kv4AttendParams& p, int d, int g, cudaStream_t stream) {
+  if (d == 64 && g == 32) return launch_one<T, 64, 32>(p, stream);
+  if (d == 64 && g == 64) return launch_one<T, 64, 64>(p, stream);
+  if (d == 128 && g == 32) return launch_one<T, 128, 32>(p, stream);
+  if (d == 128 && g == 64) return launch_one<T, 128, 64>(p, stream);
+  if (d == 128 && g == 128) return launch_one<T, 128, 128>(p, stream);
+  if (d == 256 && g == 32) return launch_one<T, 256, 32>(p, stream);
+  if (d == 256 && g == 64) return launch_one<T, 256, 64>(p, stream);
+  if (d == 256 && g == 128) return launch_one<T, 256, 128>(p, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_kv4_prompt(const Kv4AttendParams& p, int f16, int d, int g, cudaStream_t stream) {
+  return f16 ? launch_shape<Kv4Fp16>(p, d, g, stream) : launch_shape<Kv4Bf16>(p, d, g, stream);
+}
+
+}  // namespace woq

@@ -111,8 +111,9 @@ def test_positions_outside_the_table(ipex):
 
 @pytest.mark.parametrize("t", [BF, FP])
 def test_values_that_are_not_finite(ipex, t):
-    """The key says it, so that rows that do not see the token are not touched; extreme finite values stay finite."""
-    d, top = 128, torch.finfo(t).max
+    """The key says it, so that rows that do not see the token are not touched; extreme finite values stay finite, and
+    come through attention: bf16 ones below 2^61, beyond which they count as not finite."""
+    d, top = 128, 2.0 ** 60.5 if t == BF else torch.finfo(t).max
     k, v = randn(1, 5, 1, d).to(t), randn(2, 5, 1, d).to(t)
     k[0, 0, 3], v[1, 0, 100], k[2, 0, 0] = math.nan, math.inf, -math.inf
     k[3, 0, 0], k[3, 0, 1], v[3, 0, 64], v[3, 0, 65] = top, -top, -top, top
@@ -124,6 +125,19 @@ def test_values_that_are_not_finite(ipex, t):
     assert torch.equal(vv[[0, 2]].double(), R.quantise(v[[0, 2]], 64)[0])
     assert torch.equal(kk[[3, 4]].double(), R.quantise(k[[3, 4]], 64)[0]) and kk[3].isfinite().all()
     assert torch.equal(vv[[3, 4]].double(), R.quantise(v[[3, 4]], 64)[0]) and vv[3:].isfinite().all()
+    if t == BF:
+        k3 = randn(5, 2, 1, d).to(t)
+        k3[1, 0, 9] = 2.0 ** 61
+        c.append(k3.cuda(), k3.flip(0).cuda(), torch.arange(5, 7).cuda())
+        kk, vv = (x.cpu() for x in c.read(torch.arange(5, 7).cuda()))
+        assert kk.isnan().all() and (vv[0] == 0).all() and torch.equal(vv[1].double(), R.quantise(k3[:1], 64)[0][0])
+    # the extreme values: one key each, so that the output is the value
+    for i in (3, 4):
+        table = torch.zeros(1, 1).int().cuda()
+        c.append(torch.zeros(1, 1, d, dtype=t, device="cuda"), v[i:i + 1].cuda(), torch.zeros(1).long().cuda())
+        o = c.attention(torch.ones(1, 2, d, dtype=t, device="cuda"), table, torch.tensor([1]).int().cuda())
+        want = R.quantise(v[i:i + 1], 64)[0]
+        assert ((o.cpu().double() - want).abs() <= want.abs() * 2.0 ** -20).all()
     # queries of 2 tokens: the first does not see token 4 (made NaN), the second does
     k2 = randn(3, 5, 1, d).to(t)
     v2 = k2.clone()
