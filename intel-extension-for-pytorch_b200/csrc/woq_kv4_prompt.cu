@@ -4,8 +4,8 @@
 // A CTA takes one kv head of one sequence and NQ tiles of 128 query rows (a row is a token's query head; the heads
 // of a kv head lie next to one another, so they share its keys), and walks over the keys in tiles of KT:
 //   warps 0 .. 4 NQ - 1   softmax: thread = query row.  Scores from tensor memory, probabilities back over them
-//   4 warps               keys:   codes of a tile to T in shared memory, K-major with 128-byte swizzle
-//   4 warps               values: the same, transposed (a row per element, its keys next to one another)
+//   4 warps               codes of a tile to T in shared memory, K-major with 128-byte swizzle; values transposed (a row
+//                         per element, its keys next to one another)
 //   1 warp                issues S = Q K^T and O += P V; allocates tensor memory
 // The products of one tile of rows run while the other tile's softmax does.  Codes are loaded straight into
 // registers, one tile ahead; the dequantised values (bf16: times 2^-64, see Dequant) never leave the SM.
@@ -25,10 +25,11 @@ struct Shape {
   static constexpr int kNQ = D == 256 ? 1 : 2;    // tiles of 128 rows
   static constexpr int kKeys = D == 256 ? 64 : 128;
   static constexpr int kRows = 128 * kNQ;
-  static constexpr int kSoftmaxWarps = 4 * kNQ, kKeyWarp0 = kSoftmaxWarps, kValueWarp0 = kKeyWarp0 + 4, kMmaWarp = kValueWarp0 + 4;
+  static constexpr int kSoftmaxWarps = 4 * kNQ, kDequantWarp0 = kSoftmaxWarps, kMmaWarp = kDequantWarp0 + 4;
   static constexpr int kThreads = (kMmaWarp + 1) * 32;
   static constexpr int kQBytes = 128 * D * 2, kKBytes = kKeys * D * 2;  // of a tile of queries, of keys or values
-  static constexpr int q = 1024, k = q + kNQ * kQBytes, v = k + 2 * kKBytes, total = v + 2 * kKBytes + 1024;
+  static constexpr int q = 1024, k = q + kNQ * kQBytes, v = k + 2 * kKBytes, used = v + 2 * kKBytes + 1024;
+  static constexpr int total = used < 116 * 1024 ? 116 * 1024 : used;  // one CTA an SM: it takes all of tensor memory
 };
 static_assert(Shape<64>::total <= 227 * 1024 && Shape<128>::total <= 227 * 1024 && Shape<256>::total <= 227 * 1024, "shared memory");
 
@@ -40,6 +41,33 @@ struct Header {
   int b, tile;
 };
 static_assert(sizeof(Header) <= 1024, "header");
+// two 32-bit operations an instruction
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void halves_of(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// waits for the loads issued so far; the registers pass through, so that nothing that reads them moves ahead of it
+__device__ __forceinline__ void wait_ld_x32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -65,13 +93,88 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void wait_ld_x16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+// 16 columns of scores: those of keys that the row does not see (`left` of the columns are seen) to -inf
+__device__ __forceinline__ void mask16(uint32_t (&x)[16], int left) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (e >= left) x[e] = 0xff800000u;
+}
+// Calls work(x, c) for the KT columns from t_s, 16 at a time, with the next 16 on their way.  A short loop: the roles'
+// code together has to stay in the instruction cache (unrolled, a third of all stalls were instruction fetches).
+template <int KT, typename Work>
+__device__ __forceinline__ void over_columns(uint32_t t_s, Work work) {
+  uint32_t a[16], b[16];
+  tmem_ld_x16(t_s, a);
+#pragma unroll 1
+  for (int c = 0; c < KT / 16; c += 2) {
+    wait_ld_x16(a);
+    tmem_ld_x16(t_s + (c + 1) * 16, b);
+    work(a, c);
+    wait_ld_x16(b);
+    if (c + 2 < KT / 16) tmem_ld_x16(t_s + (c + 2) * 16, a);
+    work(b, c + 1);
+  }
+}
+// the largest score of a row; `sees`: how many of the tile's keys the row sees, `gone`: blocks of 16 that do not exist
+template <int KT, bool MASKED>
+__device__ __forceinline__ float tile_max(uint32_t t_s, int sees, uint32_t gone) {
+  float most = -INFINITY;
+  over_columns<KT>(t_s, [&](uint32_t(&x)[16], int c) {
+    if (MASKED) mask16(x, (gone >> c) & 1 ? 0 : sees - c * 16);
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) most = fmaxf(most, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+  });
+  return most;
+}
+// probabilities 2^(score * scale + base) of a row, in T over the scores; returns their sum
+template <typename T, int KT, bool MASKED>
+__device__ __forceinline__ float tile_exp(uint32_t t_s, float scale, float base, int sees, uint32_t gone) {
+  const uint64_t scale2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
+  const uint64_t base2 = pair_of(__float_as_uint(base), __float_as_uint(base));
+  uint64_t part = 0;
+  over_columns<KT>(t_s, [&](uint32_t(&x)[16], int c) {
+    if (MASKED) mask16(x, (gone >> c) & 1 ? 0 : sees - c * 16);
+    uint32_t out[8];
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) {
+      float y0, y1;
+      halves_of(fma_x2(pair_of(x[e], x[e + 1]), scale2, base2), y0, y1);
+      if (MASKED) {  // (-inf times a scale of 0)
+        if (x[e] == 0xff800000u) y0 = -INFINITY;
+        if (x[e + 1] == 0xff800000u) y1 = -INFINITY;
+      }
+      y0 = exp2_approx(y0);
+      y1 = exp2_approx(y1);
+      part = add_x2(part, pair_of(__float_as_uint(y0), __float_as_uint(y1)));
+      out[e / 2] = T::pack(y0, y1);
+    }
+    tmem_st_x8(t_s + c * 8, out);
+  });
+  float s0, s1;
+  halves_of(part, s0, s1);
+  return s0 + s1;
 }
 
 // The sequence and tile of rows of a CTA (b = batch: none), found by one warp.  A sequence's last rows see most keys:
@@ -215,23 +318,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         if (gone && lane == 0) atomicCAS(p.status, 0, kStatusBadPage);
         mbar_wait(&hd->s_full[i], j & 1, abort_flag, p.status, 920);
         tc_fence_after_sync();
-        float most = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld_x32(t_s + c * 32, r);
-          tc_wait_ld();
-          if (masked) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (key0 + c * 32 + e >= sees || ((gone >> (c * 2 + e / 16)) & 1)) r[e] = 0xff800000u;
-          }
-#pragma unroll
-          for (int e = 0; e < 32; ++e) most = fmaxf(most, __uint_as_float(r[e]));
-        }
+        // once over the tile for its maximum, once for the probabilities, which are stored over the scores that have been
+        // read; the next 16 columns are on their way while the last ones are worked on
+        float most = masked ? tile_max<KT, true>(t_s, sees - key0, gone) : tile_max<KT, false>(t_s, 0, 0);
         most *= scale;  // (NaN for a row that sees nothing of the tile at a scale of 0: ignored)
         if (__any_sync(0xffffffffu, most - top > 8.f)) {
-          const float m = fmaxf(most, top), f = top == m ? 1.f : exp2f(top - m);
+          const float m = fmaxf(most, top), f = top == m ? 1.f : exp2_approx(top - m);
           top = m;
           sum *= f;
           if (j > 0) {
@@ -239,36 +331,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
             tc_fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
-              uint32_t r[32];
-              tmem_ld_x32(t_o + c * 32, r);
-              tc_wait_ld();
+              uint32_t x[32];
+              tmem_ld_x32(t_o + c * 32, x);
+              wait_ld_x32(x);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
-              tmem_st_x32(t_o + c * 32, r);
+              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+              tmem_st_x32(t_o + c * 32, x);
             }
           }
         }
-        const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int c = 0; c < KT / 32; ++c) {
-          uint32_t r[32], out[16];
-          tmem_ld_x32(t_s + c * 32, r);
-          tc_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float x = fmaf(__uint_as_float(r[e]), scale, -base), y = fmaf(__uint_as_float(r[e + 1]), scale, -base);
-            if (masked) {
-              const bool no = (gone >> (c * 2 + e / 16)) & 1;
-              if (no || key0 + c * 32 + e >= sees) x = -INFINITY;
-              if (no || key0 + c * 32 + e + 1 >= sees) y = -INFINITY;
-            }
-            x = exp2_approx(x);
-            y = exp2_approx(y);
-            sum += x + y;
-            out[e / 2] = T::pack(x, y);
-          }
-          tmem_st_x16(t_s + c * 16, out);
-        }
+        const float base = top == -INFINITY ? 0.f : -top;
+        sum += masked ? tile_exp<T, KT, true>(t_s, scale, base, sees - key0, gone) : tile_exp<T, KT, false>(t_s, scale, base, 0, 0);
         tc_wait_st();
         tc_fence_before_sync();
         mbar_arrive(&hd->p_full[i]);
@@ -287,7 +360,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         uint32_t r[32];
         if (n > 0) {
           tmem_ld_x32(t_o + c * 32, r);
-          tc_wait_ld();
+          wait_ld_x32(r);
         }
         if (row < rows) {
 #pragma unroll
@@ -301,33 +374,32 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         }
       }
       tc_fence_before_sync();
-    } else if (warp < S::kValueWarp0) {
-      // ==== keys: a thread has words [t][..] of four rows (and halves) of a tile ====
-      // lanes: 8 rows x 4 words, so that eight lanes of one t write eight rows' chunks to different banks
+    } else if (warp < S::kMmaWarp) {
+      const int dw = warp - S::kDequantWarp0;
+      // ==== keys: a thread has words [t][..] of four rows (and halves) of a tile.  Lanes: 8 rows x 4 words, so that eight
+      // lanes of one t write eight rows' chunks to different banks ====
       constexpr int kItems = KT * 4 * kHalves / 128;
-      const int kw = warp - S::kKeyWarp0;
-      uint32_t w[kItems][nw], par[kItems][kGroups];
-      auto row_of = [&](int it) { return (it / kHalves * 4 + kw) * 8 + (lane & 7); };
+      uint32_t kw[kItems][nw], kpar[kItems][kGroups];
+      auto row_of = [&](int it) { return (it / kHalves * 4 + dw) * 8 + (lane & 7); };
       const int t = lane >> 3;
-      auto load = [&](int j) {
+      auto load_keys = [&](int j) {
 #pragma unroll
         for (int it = 0; it < kItems; ++it) {
           const int key = j * KT + row_of(it), hh = it % kHalves;
           const uint8_t* blk = key < len ? block_of(key) : nullptr;
           const int r = key % kKv4Tokens;
           if (blk) {
-            load_words(blk + r * (D / 2) + hh * 64 + t * nw * 4, w[it]);
-            load_words(blk + kv4_key_params(D) + (r * ng + hh * kGroups) * 4, par[it]);
+            load_words(blk + r * (D / 2) + hh * 64 + t * nw * 4, kw[it]);
+            load_words(blk + kv4_key_params(D) + (r * ng + hh * kGroups) * 4, kpar[it]);
           } else {
 #pragma unroll
-            for (int k = 0; k < nw; ++k) w[it][k] = 0;
+            for (int k = 0; k < nw; ++k) kw[it][k] = 0;
 #pragma unroll
-            for (int k = 0; k < kGroups; ++k) par[it][k] = 0;
+            for (int k = 0; k < kGroups; ++k) kpar[it][k] = 0;
           }
         }
       };
-      if (n_max > 0) load(0);
-      for (int j = 0; j < n_max; ++j) {
+      auto put_keys = [&](int j) {
         uint8_t* dst = smem + S::k + (j & 1) * S::kKBytes;
         if (j >= 2) mbar_wait(&hd->k_empty[j & 1], ((j >> 1) - 1) & 1, abort_flag, p.status, 923);
 #pragma unroll
@@ -336,9 +408,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
           Dequant<T> dq;
 #pragma unroll
           for (int k = 0; k < nw; ++k) {
-            if (k % kWordsPerGroup == 0) dq.same(par[it][k / kWordsPerGroup]);
+            if (k % kWordsPerGroup == 0) dq.same(kpar[it][k / kWordsPerGroup]);
             uint32_t x[4];
-            dq.values(w[it][k], x);
+            dq.values(kw[it][k], x);
             const int ch = hh * 16 + 4 * k + t;  // 8 elements from 8 ch
             *reinterpret_cast<uint4*>(dst + (ch >> 3) * (KT * 128) + row * 128 + (((ch & 7) ^ (row & 7)) << 4)) =
                 make_uint4(x[0], x[1], x[2], x[3]);
@@ -346,38 +418,35 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         }
         fence_async_proxy();
         mbar_arrive(&hd->k_full[j & 1]);
-        if (j + 1 < n_max) load(j + 1);
-      }
-    } else if (warp < S::kMmaWarp) {
+      };
       // ==== values: a thread has elements g + 8 n + 32 k (of a half) of eight tokens of a tile ====
-      const int id = (warp - S::kValueWarp0) * 4 + (lane >> 3), g = lane & 7;
+      const int id = dw * 4 + (lane >> 3), g = lane & 7;
       const int hh = id % kHalves, eight = id / kHalves;  // half of the head, eight tokens
-      uint32_t w[4][nw], par[8][kGroups];
-      auto load = [&](int j) {
+      uint32_t vw[4][nw], vpar[8][kGroups];
+      auto load_values = [&](int j) {
         const int key = j * KT + eight * 8;
         const uint8_t* blk = key < len ? block_of(key) : nullptr;
         const int p0 = (eight & 1) * 4;  // first pair of tokens in its block
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (blk) {
-            load_words(blk + 8 * D + hh * W * 8 + (g * 8 + ((p0 + k) ^ kv4_swap(D, g))) * (nw * 4), w[k]);
+            load_words(blk + 8 * D + hh * W * 8 + (g * 8 + ((p0 + k) ^ kv4_swap(D, g))) * (nw * 4), vw[k]);
           } else {
 #pragma unroll
-            for (int e = 0; e < nw; ++e) w[k][e] = 0;
+            for (int e = 0; e < nw; ++e) vw[k][e] = 0;
           }
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           if (blk && key + k < len) {
-            load_words(blk + kv4_value_params(D, G) + ((p0 * 2 + k) * ng + hh * kGroups) * 4, par[k]);
+            load_words(blk + kv4_value_params(D, G) + ((p0 * 2 + k) * ng + hh * kGroups) * 4, vpar[k]);
           } else {
 #pragma unroll
-            for (int e = 0; e < kGroups; ++e) par[k][e] = 0;  // tokens behind the last one hold anything
+            for (int e = 0; e < kGroups; ++e) vpar[k][e] = 0;  // tokens behind the last one hold anything
           }
         }
       };
-      if (n_max > 0) load(0);
-      for (int j = 0; j < n_max; ++j) {
+      auto put_values = [&](int j) {
         uint8_t* dst = smem + S::v + (j & 1) * S::kKBytes;
         if (j >= 2) mbar_wait(&hd->v_empty[j & 1], ((j >> 1) - 1) & 1, abort_flag, p.status, 924);
         Dequant<T> dq[4];
@@ -385,11 +454,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         for (int k = 0; k < nw; ++k) {
           if (k % kWordsPerGroup == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dq[e].pair(par[2 * e][k / kWordsPerGroup], par[2 * e + 1][k / kWordsPerGroup]);
+            for (int e = 0; e < 4; ++e) dq[e].pair(vpar[2 * e][k / kWordsPerGroup], vpar[2 * e + 1][k / kWordsPerGroup]);
           }
           uint32_t x[4][4];  // [pair of tokens][n]
 #pragma unroll
-          for (int e = 0; e < 4; ++e) dq[e].values(w[e][k], x[e]);
+          for (int e = 0; e < 4; ++e) dq[e].values(vw[e][k], x[e]);
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             const int d = hh * 128 + 32 * k + 8 * n + g;
@@ -399,43 +468,65 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         }
         fence_async_proxy();
         mbar_arrive(&hd->v_full[j & 1]);
-        if (j + 1 < n_max) load(j + 1);
+      };
+      // (the first keys' products start while the values are on their way; later loads are a tile ahead)
+      if (n_max > 0) {
+        load_keys(0);
+        load_values(0);
+        put_keys(0);
+        if (n_max > 1) load_keys(1);
+      }
+#pragma unroll 1
+      for (int j = 0; j < n_max; ++j) {
+        if (j + 1 < n_max) put_keys(j + 1);
+        if (j + 2 < n_max) load_keys(j + 2);
+        put_values(j);
+        if (j + 1 < n_max) load_values(j + 1);
       }
     } else {
       if (lane == 0) {
       // ==== products ====
       const uint32_t id_s = umma_idesc(KT, kFormat, kFormat, 1), id_o = umma_idesc(D, kFormat, kFormat, 1);
       const uint32_t q_base = smem_u32(smem + S::q), k_base = smem_u32(smem + S::k), v_base = smem_u32(smem + S::v);
+      // (a descriptor's low bits are the address / 16)
       auto scores = [&](int i, int j) {
+        const uint64_t q_desc = umma_desc_k128(q_base + i * S::kQBytes), k_desc = umma_desc_k128(k_base + (j & 1) * S::kKBytes);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          umma_f16_ss(tmem + i * 256, umma_desc_k128(q_base + i * S::kQBytes + (s >> 2) * (128 * 128) + (s & 3) * 32),
-                      umma_desc_k128(k_base + (j & 1) * S::kKBytes + (s >> 2) * (KT * 128) + (s & 3) * 32), id_s, s > 0);
+          umma_f16_ss(tmem + i * 256, q_desc + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16,
+                      k_desc + ((s >> 2) * (KT * 128) + (s & 3) * 32) / 16, id_s, s > 0);
         tc_commit(&hd->s_full[i]);
       };
+      auto values = [&](int i, int j) {
+        const uint64_t v_desc = umma_desc_k128(v_base + (j & 1) * S::kKBytes);
+#pragma unroll
+        for (int s = 0; s < KT / 16; ++s)
+          umma_f16_ts(tmem + i * 256 + 128, tmem + i * 256 + s * 8, v_desc + ((s >> 2) * (D * 128) + (s & 3) * 32) / 16, id_o,
+                      j > 0 || s > 0);
+        tc_commit(&hd->o_full[i]);
+      };
+      const int n0 = tiles_of[0], n1 = tiles_of[NQ - 1];
       if (n_max > 0) {
         mbar_wait(&hd->k_full[0], 0, abort_flag, p.status, 925);
         tc_fence_after_sync();
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < NQ; ++i)
-          if (tiles_of[i] > 0) scores(i, 0);
+          if ((i ? n1 : n0) > 0) scores(i, 0);
         tc_commit(&hd->k_empty[0]);
       }
+#pragma unroll 1
       for (int j = 0; j < n_max; ++j) {
         mbar_wait(&hd->v_full[j & 1], (j >> 1) & 1, abort_flag, p.status, 926);
         if (j + 1 < n_max) mbar_wait(&hd->k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag, p.status, 927);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < NQ; ++i) {
-          if (j < tiles_of[i]) {
+          const int n = i ? n1 : n0;
+          if (j < n) {
             mbar_wait(&hd->p_full[i], j & 1, abort_flag, p.status, 928);
             tc_fence_after_sync();
-#pragma unroll
-            for (int s = 0; s < KT / 16; ++s)
-              umma_f16_ts(tmem + i * 256 + 128, tmem + i * 256 + s * 8,
-                          umma_desc_k128(v_base + (j & 1) * S::kKBytes + (s >> 2) * (D * 128) + (s & 3) * 32), id_o, j > 0 || s > 0);
-            tc_commit(&hd->o_full[i]);
+            values(i, j);
           }
-          if (j + 1 < tiles_of[i]) scores(i, j + 1);
+          if (j + 1 < n) scores(i, j + 1);
         }
         tc_commit(&hd->v_empty[j & 1]);
         if (j + 1 < n_max) tc_commit(&hd->k_empty[(j + 1) & 1]);
