@@ -35,7 +35,7 @@ static_assert(Shape<64>::total <= 227 * 1024 && Shape<128>::total <= 227 * 1024 
 
 struct Header {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_full[2], o_full[2], q_full;
   uint32_t tmem;
   int abort_flag;
   int b, tile;
@@ -71,14 +71,36 @@ __device__ __forceinline__ void wait_ld_x32(uint32_t (&r)[32]) {
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// Products and commits of one thread, written for a whole warp: `one` is set in one of its lanes.  The warp stays together,
+// so that descriptors live in uniform registers; in a branch of a single lane each product cost eight moves to them.
+__device__ __forceinline__ void umma_f16_ss_one(uint32_t one, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                                uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :
-      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts_one(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                                uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      :
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void commit_one(uint32_t one, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(one)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -93,47 +115,33 @@ __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
-               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-__device__ __forceinline__ void wait_ld_x16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-}
-
-// 16 columns of scores: those of keys that the row does not see (`left` of the columns are seen) to -inf
-__device__ __forceinline__ void mask16(uint32_t (&x)[16], int left) {
+// 32 columns of scores: those of keys that the row does not see to -inf
+__device__ __forceinline__ void mask32(uint32_t (&x)[32], int sees, uint32_t gone) {
 #pragma unroll
-  for (int e = 0; e < 16; ++e)
-    if (e >= left) x[e] = 0xff800000u;
+  for (int e = 0; e < 32; ++e)
+    if (e >= sees || ((gone >> (e / 16)) & 1)) x[e] = 0xff800000u;
 }
-// Calls work(x, c) for the KT columns from t_s, 16 at a time, with the next 16 on their way.  A short loop: the roles'
+// Calls work(x, c) for the KT columns from t_s, 32 at a time, with the next 32 on their way.  A short loop: the roles'
 // code together has to stay in the instruction cache (unrolled, a third of all stalls were instruction fetches).
 template <int KT, typename Work>
 __device__ __forceinline__ void over_columns(uint32_t t_s, Work work) {
-  uint32_t a[16], b[16];
-  tmem_ld_x16(t_s, a);
+  uint32_t a[32], b[32];
+  tmem_ld_x32(t_s, a);
 #pragma unroll 1
-  for (int c = 0; c < KT / 16; c += 2) {
-    wait_ld_x16(a);
-    tmem_ld_x16(t_s + (c + 1) * 16, b);
+  for (int c = 0; c < KT / 32; c += 2) {
+    wait_ld_x32(a);
+    tmem_ld_x32(t_s + (c + 1) * 32, b);
     work(a, c);
-    wait_ld_x16(b);
-    if (c + 2 < KT / 16) tmem_ld_x16(t_s + (c + 2) * 16, a);
+    wait_ld_x32(b);
+    if (c + 2 < KT / 32) tmem_ld_x32(t_s + (c + 2) * 32, a);
     work(b, c + 1);
   }
 }
@@ -141,10 +149,10 @@ __device__ __forceinline__ void over_columns(uint32_t t_s, Work work) {
 template <int KT, bool MASKED>
 __device__ __forceinline__ float tile_max(uint32_t t_s, int sees, uint32_t gone) {
   float most = -INFINITY;
-  over_columns<KT>(t_s, [&](uint32_t(&x)[16], int c) {
-    if (MASKED) mask16(x, (gone >> c) & 1 ? 0 : sees - c * 16);
+  over_columns<KT>(t_s, [&](uint32_t(&x)[32], int c) {
+    if (MASKED) mask32(x, sees - c * 32, gone >> (2 * c));
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) most = fmaxf(most, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
+    for (int e = 0; e < 32; e += 2) most = fmaxf(most, fmaxf(__uint_as_float(x[e]), __uint_as_float(x[e + 1])));
   });
   return most;
 }
@@ -154,11 +162,11 @@ __device__ __forceinline__ float tile_exp(uint32_t t_s, float scale, float base,
   const uint64_t scale2 = pair_of(__float_as_uint(scale), __float_as_uint(scale));
   const uint64_t base2 = pair_of(__float_as_uint(base), __float_as_uint(base));
   uint64_t part = 0;
-  over_columns<KT>(t_s, [&](uint32_t(&x)[16], int c) {
-    if (MASKED) mask16(x, (gone >> c) & 1 ? 0 : sees - c * 16);
-    uint32_t out[8];
+  over_columns<KT>(t_s, [&](uint32_t(&x)[32], int c) {
+    if (MASKED) mask32(x, sees - c * 32, gone >> (2 * c));
+    uint32_t out[16];
 #pragma unroll
-    for (int e = 0; e < 16; e += 2) {
+    for (int e = 0; e < 32; e += 2) {
       float y0, y1;
       halves_of(fma_x2(pair_of(x[e], x[e + 1]), scale2, base2), y0, y1);
       if (MASKED) {  // (-inf times a scale of 0)
@@ -170,7 +178,7 @@ __device__ __forceinline__ float tile_exp(uint32_t t_s, float scale, float base,
       part = add_x2(part, pair_of(__float_as_uint(y0), __float_as_uint(y1)));
       out[e / 2] = T::pack(y0, y1);
     }
-    tmem_st_x8(t_s + c * 8, out);
+    tmem_st_x16(t_s + c * 16, out);
   });
   float s0, s1;
   halves_of(part, s0, s1);
@@ -234,6 +242,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       mbar_init(&hd->p_full[i], 128);
       mbar_init(&hd->o_full[i], 1);
     }
+    mbar_init(&hd->q_full, S::kRows);
     mbar_fence_init();
     hd->abort_flag = 0;
   }
@@ -268,37 +277,30 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       n_max = max(n_max, tiles_of[i]);
     }
     const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_ld;
-    // the block that holds key `key` < len of this head; null: its page does not exist
-    auto block_of = [&](int key) -> const uint8_t* {
-      const int blk = key / kKv4Tokens, page_at = p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks;
-      const int page = table[page_at], inner = blk - page_at * p.page_blocks;
-      if (page < 0 || page >= p.num_pages) return nullptr;
-      return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + h) * p.page_blocks + inner) * kBlock;
-    };
-
-    // ---- queries: K-major, 64 elements a 128-byte row, 16-byte chunks swizzled ----
-    for (int i = threadIdx.x; i < kRows * (D / 8); i += S::kThreads) {
-      const int row = i / (D / 8), ch = i % (D / 8), at = row_base + row;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (at < rows)
-        x = *reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(q0 + at / p.heads) * p.q_tok +
-                                            static_cast<int64_t>(h * p.heads + at % p.heads) * p.q_head + ch * 8);
-      if (p.scale < 0.f) {  // the sign of the scale, so that the largest product is the largest score
-        x.x ^= 0x80008000u;
-        x.y ^= 0x80008000u;
-        x.z ^= 0x80008000u;
-        x.w ^= 0x80008000u;
-      }
-      const int r = row & 127;
-      *reinterpret_cast<uint4*>(smem + S::q + (row >> 7) * S::kQBytes + (ch >> 3) * (128 * 128) + r * 128 +
-                                (((ch & 7) ^ (r & 7)) << 4)) = x;
-    }
-    fence_async_proxy();
-    __syncthreads();
 
     if (warp < S::kSoftmaxWarps) {
       // ==== softmax ====
       const int i = warp >> 2, quarter = warp & 3, row = row_base + i * 128 + quarter * 32 + lane;
+      {
+        // ---- the thread's query row: K-major, 64 elements a 128-byte row, 16-byte chunks swizzled ----
+        const int r = quarter * 32 + lane, token = row / p.heads;
+        const uint16_t* src = p.q + static_cast<int64_t>(q0 + token) * p.q_tok + static_cast<int64_t>(h * p.heads + row - token * p.heads) * p.q_head;
+        const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;  // the scale's, so that the largest product is the largest score
+        uint8_t* dst = smem + S::q + i * S::kQBytes + r * 128;
+#pragma unroll
+        for (int c0 = 0; c0 < D / 8; c0 += 8) {
+          uint4 x[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            x[c] = row < rows ? *reinterpret_cast<const uint4*>(src + (c0 + c) * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<uint4*>(dst + (c0 >> 3) * (128 * 128) + ((c ^ (r & 7)) << 4)) =
+                make_uint4(x[c].x ^ sign, x[c].y ^ sign, x[c].z ^ sign, x[c].w ^ sign);
+        }
+        fence_async_proxy();
+        mbar_arrive(&hd->q_full);
+      }
       const uint32_t t_s = tmem + i * 256 + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 128;
       const int n = NQ == 1 || i == 0 ? tiles_of[0] : tiles_of[NQ - 1];
       int sees = p.causal ? len - n_tok + row / p.heads + 1 : len;
@@ -309,11 +311,19 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       for (int o = 16; o > 0; o >>= 1) all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, o));
       const float scale = fabsf(p.scale);
       float top = -INFINITY, sum = 0.f;
+      // the pages of a tile's blocks, a tile ahead: keys of pages that do not exist are masked
+      auto fetch_page = [&](int j) -> int {
+        const int key = j * KT + lane * kKv4Tokens, blk = key / kKv4Tokens;
+        if (lane >= KT / kKv4Tokens || key >= len) return 0;
+        return table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
+      };
+      int page = fetch_page(0);
+#pragma unroll 1
       for (int j = 0; j < n; ++j) {
         const int key0 = j * KT;
-        uint32_t gone = 0;  // blocks of the tile whose page does not exist
-        if (key0 + lane * kKv4Tokens < len && lane < KT / kKv4Tokens) gone = block_of(key0 + lane * kKv4Tokens) == nullptr;
-        gone = __ballot_sync(0xffffffffu, gone);
+        const int next_page = fetch_page(j + 1);
+        const uint32_t gone = __ballot_sync(0xffffffffu, page < 0 || (page >= p.num_pages && key0 + lane * kKv4Tokens < len && lane < KT / kKv4Tokens));
+        page = next_page;
         const bool masked = key0 + KT > all_see || gone;
         if (gone && lane == 0) atomicCAS(p.status, 0, kStatusBadPage);
         mbar_wait(&hd->s_full[i], j & 1, abort_flag, p.status, 920);
@@ -376,18 +386,30 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       tc_fence_before_sync();
     } else if (warp < S::kMmaWarp) {
       const int dw = warp - S::kDequantWarp0;
+      // lane i < KT / 16 has the page of block i of a tile; fetched a tile before it is needed
+      auto fetch_pages = [&](int j) -> int {
+        const int key = j * KT + lane * kKv4Tokens, blk = key / kKv4Tokens;
+        if (lane >= KT / kKv4Tokens || key >= len) return -1;
+        return table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
+      };
+      // block `at` of tile j (for key `at` < len); null: no key, or its page does not exist
+      auto block_at = [&](int pages, int j, int at) -> const uint8_t* {
+        const int page = __shfl_sync(0xffffffffu, pages, at), blk = j * (KT / kKv4Tokens) + at;
+        if (page < 0 || page >= p.num_pages) return nullptr;
+        const int inner = p.page_shift >= 0 ? blk & (p.page_blocks - 1) : blk % p.page_blocks;
+        return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + h) * p.page_blocks + inner) * kBlock;
+      };
       // ==== keys: a thread has words [t][..] of four rows (and halves) of a tile.  Lanes: 8 rows x 4 words, so that eight
       // lanes of one t write eight rows' chunks to different banks ====
       constexpr int kItems = KT * 4 * kHalves / 128;
       uint32_t kw[kItems][nw], kpar[kItems][kGroups];
       auto row_of = [&](int it) { return (it / kHalves * 4 + dw) * 8 + (lane & 7); };
       const int t = lane >> 3;
-      auto load_keys = [&](int j) {
+      auto load_keys = [&](int j, int pages) {
 #pragma unroll
         for (int it = 0; it < kItems; ++it) {
-          const int key = j * KT + row_of(it), hh = it % kHalves;
-          const uint8_t* blk = key < len ? block_of(key) : nullptr;
-          const int r = key % kKv4Tokens;
+          const int hh = it % kHalves, r = row_of(it) % kKv4Tokens;
+          const uint8_t* blk = block_at(pages, j, row_of(it) / kKv4Tokens);
           if (blk) {
             load_words(blk + r * (D / 2) + hh * 64 + t * nw * 4, kw[it]);
             load_words(blk + kv4_key_params(D) + (r * ng + hh * kGroups) * 4, kpar[it]);
@@ -423,9 +445,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       const int id = dw * 4 + (lane >> 3), g = lane & 7;
       const int hh = id % kHalves, eight = id / kHalves;  // half of the head, eight tokens
       uint32_t vw[4][nw], vpar[8][kGroups];
-      auto load_values = [&](int j) {
+      auto load_values = [&](int j, int pages) {
         const int key = j * KT + eight * 8;
-        const uint8_t* blk = key < len ? block_of(key) : nullptr;
+        const uint8_t* blk = block_at(pages, j, eight >> 1);
         const int p0 = (eight & 1) * 4;  // first pair of tokens in its block
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -470,22 +492,25 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         mbar_arrive(&hd->v_full[j & 1]);
       };
       // (the first keys' products start while the values are on their way; later loads are a tile ahead)
+      int pages0 = fetch_pages(0), pages1 = fetch_pages(1), pages2 = -1;  // of tiles j, j + 1, j + 2
       if (n_max > 0) {
-        load_keys(0);
-        load_values(0);
+        load_keys(0, pages0);
+        load_values(0, pages0);
         put_keys(0);
-        if (n_max > 1) load_keys(1);
+        if (n_max > 1) load_keys(1, pages1);
       }
 #pragma unroll 1
       for (int j = 0; j < n_max; ++j) {
+        pages2 = fetch_pages(j + 2);
         if (j + 1 < n_max) put_keys(j + 1);
-        if (j + 2 < n_max) load_keys(j + 2);
+        if (j + 2 < n_max) load_keys(j + 2, pages2);
         put_values(j);
-        if (j + 1 < n_max) load_values(j + 1);
+        if (j + 1 < n_max) load_values(j + 1, pages1);
+        pages1 = pages2;
       }
     } else {
-      if (lane == 0) {
       // ==== products ====
+      const uint32_t one = lane == 0;
       const uint32_t id_s = umma_idesc(KT, kFormat, kFormat, 1), id_o = umma_idesc(D, kFormat, kFormat, 1);
       const uint32_t q_base = smem_u32(smem + S::q), k_base = smem_u32(smem + S::k), v_base = smem_u32(smem + S::v);
       // (a descriptor's low bits are the address / 16)
@@ -493,26 +518,27 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         const uint64_t q_desc = umma_desc_k128(q_base + i * S::kQBytes), k_desc = umma_desc_k128(k_base + (j & 1) * S::kKBytes);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          umma_f16_ss(tmem + i * 256, q_desc + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16,
+          umma_f16_ss_one(one, tmem + i * 256, q_desc + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16,
                       k_desc + ((s >> 2) * (KT * 128) + (s & 3) * 32) / 16, id_s, s > 0);
-        tc_commit(&hd->s_full[i]);
+        commit_one(one, &hd->s_full[i]);
       };
       auto values = [&](int i, int j) {
         const uint64_t v_desc = umma_desc_k128(v_base + (j & 1) * S::kKBytes);
 #pragma unroll
         for (int s = 0; s < KT / 16; ++s)
-          umma_f16_ts(tmem + i * 256 + 128, tmem + i * 256 + s * 8, v_desc + ((s >> 2) * (D * 128) + (s & 3) * 32) / 16, id_o,
+          umma_f16_ts_one(one, tmem + i * 256 + 128, tmem + i * 256 + s * 8, v_desc + ((s >> 2) * (D * 128) + (s & 3) * 32) / 16, id_o,
                       j > 0 || s > 0);
-        tc_commit(&hd->o_full[i]);
+        commit_one(one, &hd->o_full[i]);
       };
       const int n0 = tiles_of[0], n1 = tiles_of[NQ - 1];
       if (n_max > 0) {
+        mbar_wait(&hd->q_full, 0, abort_flag, p.status, 930);
         mbar_wait(&hd->k_full[0], 0, abort_flag, p.status, 925);
         tc_fence_after_sync();
 #pragma unroll 1
         for (int i = 0; i < NQ; ++i)
           if ((i ? n1 : n0) > 0) scores(i, 0);
-        tc_commit(&hd->k_empty[0]);
+        commit_one(one, &hd->k_empty[0]);
       }
 #pragma unroll 1
       for (int j = 0; j < n_max; ++j) {
@@ -528,14 +554,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
           }
           if (j + 1 < n) scores(i, j + 1);
         }
-        tc_commit(&hd->v_empty[j & 1]);
-        if (j + 1 < n_max) tc_commit(&hd->k_empty[(j + 1) & 1]);
+        commit_one(one, &hd->v_empty[j & 1]);
+        if (j + 1 < n_max) commit_one(one, &hd->k_empty[(j + 1) & 1]);
       }
       // the last commits of the barriers that nobody waits for end with the products before them
       if (n_max > 0) mbar_wait(&hd->v_empty[(n_max - 1) & 1], ((n_max - 1) >> 1) & 1, abort_flag, p.status, 929);
       tc_fence_before_sync();
-      }
-      __syncwarp();
     }
   }
   __syncthreads();
