@@ -35,9 +35,10 @@ static_assert(Shape<64>::total <= 227 * 1024 && Shape<128>::total <= 227 * 1024 
 
 struct Header {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2], q_full;
+  uint64_t s_full[2], p_full[2], o_full[2], q_full[2];
   uint32_t tmem;
   int abort_flag;
+  int bad_page;  // a page of the sequence does not exist
   int b, tile;
 };
 static_assert(sizeof(Header) <= 1024, "header");
@@ -71,36 +72,34 @@ __device__ __forceinline__ void wait_ld_x32(uint32_t (&r)[32]) {
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Products and commits of one thread, written for a whole warp: `one` is set in one of its lanes.  The warp stays together,
-// so that descriptors live in uniform registers; in a branch of a single lane each product cost eight moves to them.
-__device__ __forceinline__ void umma_f16_ss_one(uint32_t one, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                                uint32_t idesc, uint32_t accumulate) {
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ void umma_f16_ss_plain(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :
-      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void umma_f16_ts_one(uint32_t one, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                                uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_f16_ts_plain(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       :
-      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(one)
-      : "memory");
-}
-__device__ __forceinline__ void commit_one(uint32_t one, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\t"
-      "setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-      "r"(one)
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -242,9 +241,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       mbar_init(&hd->p_full[i], 128);
       mbar_init(&hd->o_full[i], 1);
     }
-    mbar_init(&hd->q_full, S::kRows);
+    for (int i = 0; i < NQ; ++i) mbar_init(&hd->q_full[i], 128);
     mbar_fence_init();
     hd->abort_flag = 0;
+    hd->bad_page = 0;
   }
   grid_launch_dependents();
   grid_dependency_wait();
@@ -281,25 +281,32 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
     if (warp < S::kSoftmaxWarps) {
       // ==== softmax ====
       const int i = warp >> 2, quarter = warp & 3, row = row_base + i * 128 + quarter * 32 + lane;
+      const int token = row / p.heads, head = h * p.heads + row - token * p.heads;
       {
-        // ---- the thread's query row: K-major, 64 elements a 128-byte row, 16-byte chunks swizzled ----
-        const int r = quarter * 32 + lane, token = row / p.heads;
-        const uint16_t* src = p.q + static_cast<int64_t>(q0 + token) * p.q_tok + static_cast<int64_t>(h * p.heads + row - token * p.heads) * p.q_head;
+        // ---- the warp's 32 query rows: K-major, 64 elements a 128-byte row, 16-byte chunks swizzled.  D / 8 lanes read a
+        // row; lane r knows where row r is ----
         const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;  // the scale's, so that the largest product is the largest score
-        uint8_t* dst = smem + S::q + i * S::kQBytes + r * 128;
-#pragma unroll
-        for (int c0 = 0; c0 < D / 8; c0 += 8) {
+        const int64_t at = row < rows ? static_cast<int64_t>(q0 + token) * p.q_tok + static_cast<int64_t>(head) * p.q_head : -1;
+        uint8_t* dst = smem + S::q + i * S::kQBytes + quarter * 32 * 128;
+        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += 8 * kAtOnce) {
           uint4 x[8];
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            x[c] = row < rows ? *reinterpret_cast<const uint4*>(src + (c0 + c) * 8) : make_uint4(0, 0, 0, 0);
+          for (int k = 0; k < 8; ++k) {
+            const int64_t from = __shfl_sync(0xffffffffu, at, (r0 + k * kAtOnce + lane / kLanes) & 31);
+            x[k] = from >= 0 ? *reinterpret_cast<const uint4*>(p.q + from + lane % kLanes * 8) : make_uint4(0, 0, 0, 0);
+          }
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<uint4*>(dst + (c0 >> 3) * (128 * 128) + ((c ^ (r & 7)) << 4)) =
-                make_uint4(x[c].x ^ sign, x[c].y ^ sign, x[c].z ^ sign, x[c].w ^ sign);
+          for (int k = 0; k < 8; ++k) {
+            const int r = r0 + k * kAtOnce + lane / kLanes, ch = lane % kLanes;
+            if (r < 32)
+              *reinterpret_cast<uint4*>(dst + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
+                  make_uint4(x[k].x ^ sign, x[k].y ^ sign, x[k].z ^ sign, x[k].w ^ sign);
+          }
         }
         fence_async_proxy();
-        mbar_arrive(&hd->q_full);
+        mbar_arrive(&hd->q_full[i]);
       }
       const uint32_t t_s = tmem + i * 256 + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + 128;
       const int n = NQ == 1 || i == 0 ? tiles_of[0] : tiles_of[NQ - 1];
@@ -311,23 +318,21 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       for (int o = 16; o > 0; o >>= 1) all_see = min(all_see, __shfl_xor_sync(0xffffffffu, all_see, o));
       const float scale = fabsf(p.scale);
       float top = -INFINITY, sum = 0.f;
-      // the pages of a tile's blocks, a tile ahead: keys of pages that do not exist are masked
-      auto fetch_page = [&](int j) -> int {
-        const int key = j * KT + lane * kKv4Tokens, blk = key / kKv4Tokens;
-        if (lane >= KT / kKv4Tokens || key >= len) return 0;
-        return table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
-      };
-      int page = fetch_page(0);
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
         const int key0 = j * KT;
-        const int next_page = fetch_page(j + 1);
-        const uint32_t gone = __ballot_sync(0xffffffffu, page < 0 || (page >= p.num_pages && key0 + lane * kKv4Tokens < len && lane < KT / kKv4Tokens));
-        page = next_page;
-        const bool masked = key0 + KT > all_see || gone;
-        if (gone && lane == 0) atomicCAS(p.status, 0, kStatusBadPage);
         mbar_wait(&hd->s_full[i], j & 1, abort_flag, p.status, 920);
         tc_fence_after_sync();
+        uint32_t gone = 0;  // blocks of the tile whose page does not exist: masked (looked up if the sequence has any)
+        if (*static_cast<volatile int*>(&hd->bad_page)) {
+          const int blk = key0 / kKv4Tokens + lane;
+          if (lane < KT / kKv4Tokens && blk * kKv4Tokens < len) {
+            const int page = table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
+            gone = page < 0 || page >= p.num_pages;
+          }
+          gone = __ballot_sync(0xffffffffu, gone);
+        }
+        const bool masked = key0 + KT > all_see || gone;
         // once over the tile for its maximum, once for the probabilities, which are stored over the scores that have been
         // read; the next 16 columns are on their way while the last ones are worked on
         float most = masked ? tile_max<KT, true>(t_s, sees - key0, gone) : tile_max<KT, false>(t_s, 0, 0);
@@ -362,9 +367,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         tc_fence_after_sync();
       }
       const float inv = sum == 0.f ? 0.f : Dequant<T>::kBack / sum;
-      const int token = row / p.heads;
-      uint16_t* dst = p.out + static_cast<int64_t>(q0 + token) * p.o_tok +
-                      static_cast<int64_t>(h * p.heads + row - token * p.heads) * p.o_head;
+      // to the place of the warp's query rows (their products are done) and from there, a row by D / 8 lanes
+      uint8_t* stage = smem + S::q + i * S::kQBytes + quarter * 32 * 128;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
@@ -372,15 +376,27 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
           tmem_ld_x32(t_o + c * 32, r);
           wait_ld_x32(r);
         }
-        if (row < rows) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t w[4];
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              w[k] = n > 0 && sum != 0.f ? T::pack(__uint_as_float(r[e * 8 + k * 2]) * inv, __uint_as_float(r[e * 8 + k * 2 + 1]) * inv) : 0u;
-            *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int k = 0; k < 4; ++k)
+            w[k] = n > 0 && sum != 0.f ? T::pack(__uint_as_float(r[e * 8 + k * 2]) * inv, __uint_as_float(r[e * 8 + k * 2 + 1]) * inv) : 0u;
+          const int ch = c * 4 + e;
+          *reinterpret_cast<uint4*>(stage + (ch >> 3) * (128 * 128) + lane * 128 + (((ch & 7) ^ (lane & 7)) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();
+      {
+        const int64_t at = row < rows ? static_cast<int64_t>(q0 + token) * p.o_tok + static_cast<int64_t>(head) * p.o_head : -1;
+        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+#pragma unroll 4
+        for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
+          const int r = r0 + lane / kLanes, ch = lane % kLanes;
+          const int64_t to = __shfl_sync(0xffffffffu, at, r);
+          const uint4 x = *reinterpret_cast<const uint4*>(stage + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+          if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + ch * 8) = x;
         }
       }
       tc_fence_before_sync();
@@ -390,7 +406,12 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       auto fetch_pages = [&](int j) -> int {
         const int key = j * KT + lane * kKv4Tokens, blk = key / kKv4Tokens;
         if (lane >= KT / kKv4Tokens || key >= len) return -1;
-        return table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
+        const int page = table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
+        if (page < 0 || page >= p.num_pages) {
+          *static_cast<volatile int*>(&hd->bad_page) = 1;
+          atomicCAS(p.status, 0, kStatusBadPage);
+        }
+        return page;
       };
       // block `at` of tile j (for key `at` < len); null: no key, or its page does not exist
       auto block_at = [&](int pages, int j, int at) -> const uint8_t* {
@@ -509,41 +530,53 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         pages1 = pages2;
       }
     } else {
-      // ==== products ====
-      const uint32_t one = lane == 0;
+      // ==== products.  The warp stays together and one lane issues: descriptors live in uniform registers ====
       const uint32_t id_s = umma_idesc(KT, kFormat, kFormat, 1), id_o = umma_idesc(D, kFormat, kFormat, 1);
-      const uint32_t q_base = smem_u32(smem + S::q), k_base = smem_u32(smem + S::k), v_base = smem_u32(smem + S::v);
+      const uint32_t t = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+      const uint64_t q_desc = umma_desc_k128(base + S::q), k_desc = umma_desc_k128(base + S::k), v_desc = umma_desc_k128(base + S::v);
+      const int n0 = __shfl_sync(0xffffffffu, tiles_of[0], 0), n1 = __shfl_sync(0xffffffffu, tiles_of[NQ - 1], 0);
+      const int n_all = max(n0, n1);
       // (a descriptor's low bits are the address / 16)
       auto scores = [&](int i, int j) {
-        const uint64_t q_desc = umma_desc_k128(q_base + i * S::kQBytes), k_desc = umma_desc_k128(k_base + (j & 1) * S::kKBytes);
+        const uint64_t q = q_desc + i * (S::kQBytes / 16), k = k_desc + (j & 1) * (S::kKBytes / 16);
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          umma_f16_ss_one(one, tmem + i * 256, q_desc + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16,
-                      k_desc + ((s >> 2) * (KT * 128) + (s & 3) * 32) / 16, id_s, s > 0);
-        commit_one(one, &hd->s_full[i]);
+          for (int s = 0; s < D / 16; ++s)
+            umma_f16_ss_plain(t + i * 256, q + ((s >> 2) * (128 * 128) + (s & 3) * 32) / 16, k + ((s >> 2) * (KT * 128) + (s & 3) * 32) / 16,
+                        id_s, s > 0);
+          tc_commit(&hd->s_full[i]);
+        }
+        __syncwarp();
       };
       auto values = [&](int i, int j) {
-        const uint64_t v_desc = umma_desc_k128(v_base + (j & 1) * S::kKBytes);
+        const uint64_t v = v_desc + (j & 1) * (S::kKBytes / 16);
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < KT / 16; ++s)
-          umma_f16_ts_one(one, tmem + i * 256 + 128, tmem + i * 256 + s * 8, v_desc + ((s >> 2) * (D * 128) + (s & 3) * 32) / 16, id_o,
-                      j > 0 || s > 0);
-        commit_one(one, &hd->o_full[i]);
+          for (int s = 0; s < KT / 16; ++s)
+            umma_f16_ts_plain(t + i * 256 + 128, t + i * 256 + s * 8, v + ((s >> 2) * (D * 128) + (s & 3) * 32) / 16, id_o, j > 0 || s > 0);
+          tc_commit(&hd->o_full[i]);
+        }
+        __syncwarp();
       };
-      const int n0 = tiles_of[0], n1 = tiles_of[NQ - 1];
-      if (n_max > 0) {
-        mbar_wait(&hd->q_full, 0, abort_flag, p.status, 930);
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit(bar);
+        __syncwarp();
+      };
+      if (n_all > 0) {
         mbar_wait(&hd->k_full[0], 0, abort_flag, p.status, 925);
-        tc_fence_after_sync();
 #pragma unroll 1
-        for (int i = 0; i < NQ; ++i)
+        for (int i = 0; i < NQ; ++i) {
+          mbar_wait(&hd->q_full[i], 0, abort_flag, p.status, 930);
+          tc_fence_after_sync();
           if ((i ? n1 : n0) > 0) scores(i, 0);
-        commit_one(one, &hd->k_empty[0]);
+        }
+        commit(&hd->k_empty[0]);
       }
 #pragma unroll 1
-      for (int j = 0; j < n_max; ++j) {
+      for (int j = 0; j < n_all; ++j) {
         mbar_wait(&hd->v_full[j & 1], (j >> 1) & 1, abort_flag, p.status, 926);
-        if (j + 1 < n_max) mbar_wait(&hd->k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag, p.status, 927);
+        if (j + 1 < n_all) mbar_wait(&hd->k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, abort_flag, p.status, 927);
 #pragma unroll 1
         for (int i = 0; i < NQ; ++i) {
           const int n = i ? n1 : n0;
@@ -554,11 +587,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
           }
           if (j + 1 < n) scores(i, j + 1);
         }
-        commit_one(one, &hd->v_empty[j & 1]);
-        if (j + 1 < n_max) commit_one(one, &hd->k_empty[(j + 1) & 1]);
+        commit(&hd->v_empty[j & 1]);
+        if (j + 1 < n_all) commit(&hd->k_empty[(j + 1) & 1]);
       }
       // the last commits of the barriers that nobody waits for end with the products before them
-      if (n_max > 0) mbar_wait(&hd->v_empty[(n_max - 1) & 1], ((n_max - 1) >> 1) & 1, abort_flag, p.status, 929);
+      if (n_all > 0) mbar_wait(&hd->v_empty[(n_all - 1) & 1], ((n_all - 1) >> 1) & 1, abort_flag, p.status, 929);
       tc_fence_before_sync();
     }
   }
