@@ -467,26 +467,43 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
   }
   if (!(ss < INFINITY)) scale = __int_as_float(0x7fc00000);  // codes cannot say it: the row's scale does
   if (tid == 0 && slice == 0) sa[m] = scale;
-  const float q_lo = ASYM ? 0.f : -128.f, q_hi = ASYM ? 255.f : 127.f;
   uint2* qr = reinterpret_cast<uint2*>(qa + m * k);
+  // The quotient by the scale's reciprocal is within 2^-15 of the true one; where that is near a tie the division decides.
+  // Adding 1.5 2^23 leaves the rounded code in the low bits.  (4096 x 8192: 54 us with divisions alone, 48 this way.)
+  const float rcp = scale > 0.f ? __frcp_rn(scale) : 0.f;
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int at = p0 + tid + i * 256;
     if (at >= p1) break;
-    uint32_t out[2] = {0u, 0u};
+    float y[8];
+    uint32_t c[8];
+    bool near_tie = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float a = __uint_as_float(h[i][j] << 16), b = __uint_as_float(h[i][j] & 0xffff0000u);
-      float ql = 0.f, qh = 0.f;
-      if (scale > 0.f) {
-        ql = fminf(fmaxf(rintf(__fdiv_rn(a, scale) + zp), q_lo), q_hi);
-        qh = fminf(fmaxf(rintf(__fdiv_rn(b, scale) + zp), q_lo), q_hi);
-      }
-      const uint32_t c = (static_cast<uint32_t>(static_cast<int>(ql)) & 0xffu) |
-                         ((static_cast<uint32_t>(static_cast<int>(qh)) & 0xffu) << 8);
-      out[j >> 1] |= c << ((j & 1) * 16);
+      y[2 * j] = __uint_as_float(h[i][j] << 16);
+      y[2 * j + 1] = __uint_as_float(h[i][j] & 0xffff0000u);
     }
-    qr[at] = make_uint2(out[0], out[1]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float t = y[j] * rcp;
+      if (ASYM) t = fminf(fmaxf(t + zp, 0.f), 255.f);
+      const float r = t + 12582912.f;
+      c[j] = __float_as_uint(r);
+      near_tie = near_tie || fabsf(t - (r - 12582912.f)) > 0.4999f;
+    }
+    if (near_tie && scale > 0.f) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float t = __fdiv_rn(y[j], scale);
+        t = ASYM ? fminf(fmaxf(t + zp, 0.f), 255.f) : fminf(fmaxf(t, -128.f), 127.f);
+        c[j] = __float_as_uint(t + 12582912.f);
+      }
+    }
+    const uint32_t lo01 = __byte_perm(c[0], c[1], 0x0040), lo23 = __byte_perm(c[2], c[3], 0x0040);
+    const uint32_t hi01 = __byte_perm(c[4], c[5], 0x0040), hi23 = __byte_perm(c[6], c[7], 0x0040);
+    uint2 out = make_uint2(__byte_perm(lo01, lo23, 0x5410), __byte_perm(hi01, hi23, 0x5410));
+    if (!(scale > 0.f)) out = make_uint2(0u, 0u);
+    qr[at] = out;
   }
 }
 
