@@ -639,6 +639,7 @@ at::Tensor kv4_cache_append(at::Tensor& cache, const at::Tensor& key, const at::
     TORCH_CHECK(cos_sin->device() == cache.device() && cos_sin->scalar_type() == at::kFloat && cos_sin->dim() == 2,
                 "WOQ: cos_sin must be fp32 [positions, rotated elements] on the cache's device");
     table = cos_sin->contiguous();
+    if (reinterpret_cast<uintptr_t>(table.data_ptr()) & 15) table = table.clone();
     pos = kv4_index(*positions, cache, at::kLong, "positions");
     TORCH_CHECK(pos.dim() == 1 && pos.size(0) == tokens, "WOQ: positions must have one entry per token");
     rot = table.size(1);

@@ -11,11 +11,31 @@ namespace woq {
 
 namespace {
 
-// a * c - b * s with an error below two units of the result's last place, whatever cancels (Kahan's difference of
-// products): rotated keys decide codes, and a product rounded on its own would move some of them.
-__device__ __forceinline__ float diff_of_products(float a, float c, float b, float s) {
-  const float p = b * s;
-  return fmaf(a, c, -p) - fmaf(b, s, -p);
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// a * c - b * s for two pairs with an error below two units of the result's last place, whatever cancels
+// (Kahan's difference of products): rotated keys decide codes, and a product rounded on its own would move some of them.
+__device__ __forceinline__ float2 diff_of_products(uint64_t a, uint64_t c, uint64_t b, uint64_t s) {
+  const uint64_t p = mul2(b, s) ^ 0x8000000080000000ull;  // -(b s)
+  return halves2(fma2(fma2(b, s, p), pair2(-1.f, -1.f), fma2(a, c, p)));
 }
 
 template <typename T>
@@ -47,10 +67,22 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&c)[8],
   }
   const uint16_t s16 = T::from_float_rz(__fdiv_rn(hi * 0.5f - lo * 0.5f, 7.5f));
   const float s = T::to_float(s16) * 0.5f, m = lo * 0.5f;
+  // The quotient by the scale's reciprocal is within 2^-19 of the true one (two roundings of a number up to 15.2): where it
+  // is that near a tie, the division decides.  Adding 1.5 2^23 leaves the rounded quotient in the low bits.
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  bool near_tie = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(x[i] * 0.5f - m, s)), 0.f), 15.f) : 0.f;
-    c[i] = static_cast<uint32_t>(static_cast<int>(q));
+    const float t = fminf(fmaf(x[i], 0.5f, -m) * inv, 15.f), r = t + 12582912.f;
+    c[i] = __float_as_uint(r) & 15u;
+    near_tie = near_tie || fabsf(t - (r - 12582912.f)) > 0.5f - 1.f / 131072.f;
+  }
+  if (near_tie && s > 0.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = fminf(__fdiv_rn(fmaf(x[i], 0.5f, -m), s), 15.f);
+      c[i] = __float_as_uint(t + 12582912.f) & 15u;
+    }
   }
   param = static_cast<uint32_t>(s16) | static_cast<uint32_t>(T::from_float(lo)) << 16;
 }
@@ -58,75 +90,109 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&c)[8],
 // One CTA per token (and part of its rows): D / 8 lanes a row, 8 elements a lane.  Rows are the query heads, then the
 // key heads, then the value heads; a thread keeps its 8 elements' angles over all rows.
 template <typename T, int D, int G>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendParams p) {
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(Kv4AppendParams p) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes, LG = G / 8, ng = D / G;
   const int64_t token = blockIdx.x;
   const int sub = threadIdx.x % kLanes, row0 = threadIdx.x / kLanes;
   grid_launch_dependents();
   grid_dependency_wait();
+  const int step = kRows * gridDim.y, start = row0 + static_cast<int>(blockIdx.y) * kRows;
+  // the first rows are on their way while slots, positions and angles are looked up
+  const uint16_t* q_src = p.q + token * p.q_tok + sub * 8;
+  const int q_last = p.q_heads - 1;
+  uint4 ahead = make_uint4(0, 0, 0, 0);
+  if (p.q_heads > 0) ahead = *reinterpret_cast<const uint4*>(q_src + min(start, q_last) * p.q_head);
   const int64_t slot = p.slots[token], pos = p.positions ? p.positions[token] : 0;
   const bool bad_pos = p.rot > 0 && (pos < 0 || pos >= p.max_pos);
   const bool store = !bad_pos && slot >= 0 && slot < p.num_slots;
-  const int rows = p.q_heads + 2 * p.kv_heads, first = p.q_heads + p.kv_heads;
 
-  // angles of the lane's elements: x[i] * c[i] + partner * s[i], the sign of s says which of the pair it is
-  float cs[8], sn[8];
+  // angles of the lane's elements: x[i] * c[i] - partner * s[i], the sign of s says which of the pair it is
+  uint64_t cs[4], sn[4];
   const int half = p.rot / 2, lane_rot = p.rot / 8;
   const bool turns = sub < lane_rot;
   if (turns && !bad_pos) {
     const float* t = p.cos_sin + pos * p.rot;
+    if (p.interleaved) {  // (table rows start at multiples of 16 bytes: rot is a multiple of 16)
+      const float4 c = *reinterpret_cast<const float4*>(t + sub * 4), s = *reinterpret_cast<const float4*>(t + half + sub * 4);
+      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int e = sub * 8 + i, at = p.interleaved ? e >> 1 : e % half;
-      cs[i] = t[at];
-      const float s = t[half + at];
-      sn[i] = (p.interleaved ? (e & 1) : e >= half) ? -s : s;
+      for (int i = 0; i < 4; ++i) {
+        cs[i] = pair2(cc[i], cc[i]);
+        sn[i] = pair2(ss[i], -ss[i]);
+      }
+    } else {
+      const bool second = sub >= lane_rot / 2;
+      const float4* c = reinterpret_cast<const float4*>(t + (second ? sub - lane_rot / 2 : sub) * 8);
+      const float4* s = reinterpret_cast<const float4*>(t + half + (second ? sub - lane_rot / 2 : sub) * 8);
+      const float sign = second ? -1.f : 1.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 a = c[i], b = s[i];
+        cs[2 * i] = pair2(a.x, a.y);
+        cs[2 * i + 1] = pair2(a.z, a.w);
+        sn[2 * i] = pair2(sign * b.x, sign * b.y);
+        sn[2 * i + 1] = pair2(sign * b.z, sign * b.w);
+      }
     }
   }
   // lane of the row that holds the partners (rotation of halves): whole lanes, since rot is a multiple of 16
   const int mate = (threadIdx.x & 31) - sub % kLanes + (sub < lane_rot / 2 ? sub + lane_rot / 2 : turns ? sub - lane_rot / 2 : sub);
 
-  const int64_t block = store ? slot / kKv4Tokens : 0;
-  const int r = store ? static_cast<int>(slot % kKv4Tokens) : 0;
+  // what a lane holds of a row, rotated
+  auto rotate = [&](const uint4& raw) -> uint4 {
+    uint4 other;
+    if (p.interleaved) {  // the neighbour within the pair
+      other = make_uint4(__byte_perm(raw.x, 0, 0x1032), __byte_perm(raw.y, 0, 0x1032), __byte_perm(raw.z, 0, 0x1032),
+                         __byte_perm(raw.w, 0, 0x1032));
+    } else {
+      other.x = __shfl_sync(0xffffffffu, raw.x, mate);
+      other.y = __shfl_sync(0xffffffffu, raw.y, mate);
+      other.z = __shfl_sync(0xffffffffu, raw.z, mate);
+      other.w = __shfl_sync(0xffffffffu, raw.w, mate);
+    }
+    if (!turns || bad_pos) return raw;
+    const uint32_t a[4] = {raw.x, raw.y, raw.z, raw.w}, b[4] = {other.x, other.y, other.z, other.w};
+    uint32_t z[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 y = diff_of_products(pair2(T::lo(a[i]), T::hi(a[i])), cs[i], pair2(T::lo(b[i]), T::hi(b[i])), sn[i]);
+      z[i] = T::pack(y.x, y.y);
+    }
+    return make_uint4(z[0], z[1], z[2], z[3]);
+  };
+  // ---- queries.  (The whole warp takes part in every round: shuffles; rows past the end repeat the last one and store
+  // nothing.)  The next round's row is on its way while this one is rotated ----
+  if (p.q_heads > 0) {
+    uint16_t* dst = p.q_out + token * p.q_heads * D + sub * 8;
+    for (int head = start; head - row0 <= q_last; head += step) {
+      const uint4 raw = ahead;
+      ahead = *reinterpret_cast<const uint4*>(q_src + min(head + step, q_last) * p.q_head);
+      uint4 out = p.rot > 0 ? rotate(raw) : raw;
+      if (bad_pos) out = make_uint4(T::kNan * 0x10001u, T::kNan * 0x10001u, T::kNan * 0x10001u, T::kNan * 0x10001u);
+      if (head <= q_last) *reinterpret_cast<uint4*>(dst + head * D) = out;
+    }
+  }
+  // ---- keys, then values ----
+  if (!store) return;  // (the token's, not the lane's)
+  const int64_t block = slot / kKv4Tokens;
+  const int r = static_cast<int>(slot % kKv4Tokens);
   const int64_t page = block / p.page_blocks, inner = block % p.page_blocks;
-
-  for (int row = row0 + static_cast<int>(blockIdx.y) * kRows; row - row0 < rows; row += kRows * gridDim.y) {
-    // (the whole warp takes part in every round: shuffles; rows past the end repeat the last one and store nothing)
+  const int rows = 2 * p.kv_heads;
+  // (CTAs that the queries leave idle first: the rounds go on where those ended)
+  for (int row = row0 + static_cast<int>((gridDim.y - 1 - blockIdx.y)) * kRows; row - row0 < rows; row += step) {
     const bool live = row < rows;
     const int rr = live ? row : rows - 1;
-    const bool is_q = rr < p.q_heads, is_k = !is_q && rr < first;
-    const int head = is_q ? rr : is_k ? rr - p.q_heads : rr - first;
-    const uint16_t* src = is_q ? p.q + token * p.q_tok + head * p.q_head
-                               : is_k ? p.k + token * p.k_tok + head * p.k_head : p.v + token * p.v_tok + head * p.v_head;
-    const uint4 raw = *reinterpret_cast<const uint4*>(src + sub * 8);
-    uint4 out = raw;
+    const bool is_k = rr < p.kv_heads;
+    const int head = is_k ? rr : rr - p.kv_heads;
+    const uint4 value = *reinterpret_cast<const uint4*>(p.v + token * p.v_tok + head * p.v_head + sub * 8);
+    uint4 raw = value;
+    if (is_k) raw = *reinterpret_cast<const uint4*>(p.k + token * p.k_tok + head * p.k_head + sub * 8);
+    if (p.rot > 0) {
+      const uint4 turned = rotate(raw);
+      if (is_k) raw = turned;
+    }
     float x[8];
     unpack8<T>(raw, x);
-    if (p.rot > 0) {
-      uint4 other;
-      if (p.interleaved) {
-        other = raw;
-      } else {
-        other.x = __shfl_sync(0xffffffffu, raw.x, mate);
-        other.y = __shfl_sync(0xffffffffu, raw.y, mate);
-        other.z = __shfl_sync(0xffffffffu, raw.z, mate);
-        other.w = __shfl_sync(0xffffffffu, raw.w, mate);
-      }
-      if (turns && !bad_pos && (is_q || is_k)) {
-        float y[8], z[8];
-        unpack8<T>(other, y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = diff_of_products(x[i], cs[i], p.interleaved ? y[i ^ 1] : y[i], sn[i]);
-        out = make_uint4(T::pack(z[0], z[1]), T::pack(z[2], z[3]), T::pack(z[4], z[5]), T::pack(z[6], z[7]));
-        unpack8<T>(out, x);
-      }
-    }
-    if (live && is_q) {
-      if (bad_pos) out = make_uint4(T::kNan * 0x10001u, T::kNan * 0x10001u, T::kNan * 0x10001u, T::kNan * 0x10001u);
-      *reinterpret_cast<uint4*>(p.q_out + (token * p.q_heads + head) * D + sub * 8) = out;
-    }
-    if (__all_sync(0xffffffffu, is_q)) continue;
-
     uint32_t c[8], param;
     bool finite;
     quantise8<T, LG>(x, c, param, finite);
@@ -134,7 +200,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendParams p) {
     // instead (its scores are NaN for the rows that see it, and only for those).
     if (is_k) {
       float y[8];
-      unpack8<T>(*reinterpret_cast<const uint4*>(p.v + token * p.v_tok + head * p.v_head + sub * 8), y);
+      unpack8<T>(value, y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) finite = finite && fabsf(y[i]) < T::kTooLarge;
     }
@@ -146,23 +212,22 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(Kv4AppendParams p) {
       for (int i = 0; i < 8; ++i) c[i] = 0;
     }
     uint8_t* blk = p.cache + ((page * p.kv_heads + head) * p.page_blocks + inner) * kv4_block_bytes(D, G);
-    const bool put = live && store;
     // four lanes 4 j .. 4 j + 3 hold elements 32 j + 8 n + g of nibble n: each leaves with two g of all four
     uint32_t w[4];
     const int n = sub & 3;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = (c[2 * i] | c[2 * i + 1] << 16) << (4 * n);
-    uint32_t give = n & 2 ? w[0] : w[2], give2 = n & 2 ? w[1] : w[3];
-    uint32_t a = (n & 2 ? w[2] : w[0]) | __shfl_xor_sync(0xffffffffu, give, 2);
-    uint32_t b = (n & 2 ? w[3] : w[1]) | __shfl_xor_sync(0xffffffffu, give2, 2);
+    const uint32_t give = n & 2 ? w[0] : w[2], give2 = n & 2 ? w[1] : w[3];
+    const uint32_t a = (n & 2 ? w[2] : w[0]) | __shfl_xor_sync(0xffffffffu, give, 2);
+    const uint32_t b = (n & 2 ? w[3] : w[1]) | __shfl_xor_sync(0xffffffffu, give2, 2);
     const uint32_t mine = (n & 1 ? b : a) | __shfl_xor_sync(0xffffffffu, n & 1 ? a : b, 1);
-    if (put && is_k) {
+    if (live && is_k) {
       uint32_t word = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) word |= c[i] << (4 * ((i >> 1) + 4 * (i & 1)));
       *reinterpret_cast<uint32_t*>(blk + kv4_key_word(D, r, sub)) = word;
       if (sub % LG == 0) *reinterpret_cast<uint32_t*>(blk + kv4_key_params(D) + (r * ng + sub / LG) * 4) = param;
-    } else if (put && !is_q) {
+    } else if (live) {
       const int g0 = 2 * n, hh = sub / 16, j = (sub % 16) / 4;
       *reinterpret_cast<uint16_t*>(blk + kv4_value_half(D, r, hh, j, g0)) = static_cast<uint16_t>(mine & 0xffffu);
       *reinterpret_cast<uint16_t*>(blk + kv4_value_half(D, r, hh, j, g0 + 1)) = static_cast<uint16_t>(mine >> 16);

@@ -77,8 +77,8 @@ int woq_b200_kv4_append(const woq_b200_kv4_desc* d, void* cache, const void* q, 
   if (tokens == 0) return WOQ_B200_OK;
   if (!slots || (d->num_pages > 0 && !cache)) return set_error(WOQ_B200_ERR_INVALID_ARG, "cache and slots must be non-null");
   if (!aligned16(cache)) return set_error(WOQ_B200_ERR_INVALID_ARG, "the cache must be 16-byte aligned");
-  if (rot > 0 && (!positions || !cos_sin || max_pos < 1))
-    return set_error(WOQ_B200_ERR_INVALID_ARG, "a rotation needs positions and a table of cosines and sines");
+  if (rot > 0 && (!positions || !cos_sin || max_pos < 1 || !aligned16(cos_sin)))
+    return set_error(WOQ_B200_ERR_INVALID_ARG, "a rotation needs positions and a 16-byte aligned table of cosines and sines");
   if (q_heads > 0) {
     if (int rc = check_rows("q", q, q_tok, q_head)) return rc;
     if (!q_out || !aligned16(q_out)) return set_error(WOQ_B200_ERR_INVALID_ARG, "q_out must be non-null and 16-byte aligned");

@@ -56,7 +56,7 @@ def append(capi, d=None, cache=FAKE, q=FAKE, q_tok=512, q_head=128, q_heads=4, k
 @pytest.mark.parametrize("bad, code", [
     (dict(cache=None), 1), (dict(cache=FAKE + 8), 1), (dict(slots=None), 1), (dict(k=None), 1), (dict(v=FAKE + 2), 1),
     (dict(k_tok=252), 1), (dict(q_head=4), 1), (dict(q=None), 1), (dict(q_out=None), 1), (dict(positions=None), 1),
-    (dict(cos_sin=None), 1), (dict(max_pos=0), 1), (dict(rot=8), 2), (dict(rot=144), 2), (dict(rot=-16), 2),
+    (dict(cos_sin=None), 1), (dict(cos_sin=FAKE + 4), 1), (dict(max_pos=0), 1), (dict(rot=8), 2), (dict(rot=144), 2), (dict(rot=-16), 2),
     (dict(tokens=-1), 1), (dict(q_heads=-1), 1), (dict(tokens=1 << 31), 1)])
 def test_appends_that_are_refused(capi, bad, code):
     assert append(capi, **bad) == code
