@@ -980,6 +980,8 @@ def main():
     ap.add_argument("--stack", default=None, nargs="?", const="all",
                     help="the Llama-3-8B-architecture decode stack (bench_stack.py); optionally batch sizes, e.g. 1,8")
     ap.add_argument("--new-tokens", type=int, default=128, help="--stack: greedy decode steps")
+    ap.add_argument("--kv-cache", choices=("bf16", "int4"), default="bf16",
+                    help="--stack: keys and values in a static bf16 cache, or in the paged 4-bit cache")
     args = ap.parse_args()
     if args.split is not None:
         from ipex_b200 import _capi

@@ -7,7 +7,9 @@ RoPE theta 5e5, vocabulary 128256 with the language-model head kept in bf16; ran
 through ipex_b200.llm.optimize (quantise, prepack, fuse: q/k/v as one concatenated linear, gate
 and up in one kernel with the silu*mul epilogue, the residual adds in the epilogues of o_proj and
 down_proj).  Attention, RMSNorm, RoPE, the embedding, the head and the arg-max are stock
-PyTorch: they are the harness, the linears are the thing measured.
+PyTorch: they are the harness, the linears are the thing measured.  With `--kv-cache int4` the
+rotation, the cache and attention are the framework's own as well: keys and values go to a paged
+4-bit cache (group 64) that prompts and decode steps attend to.
 
 For each batch size the prompt is prefilled into a static KV cache, then 128 greedy tokens are
 decoded with one CUDA graph per decode step replayed once per token.  Reported per batch size:
@@ -26,6 +28,7 @@ from torch import nn
 HIDDEN, LAYERS, HEADS, KV_HEADS, HEAD_DIM, FFN, VOCAB = 4096, 32, 32, 8, 128, 14336, 128256
 EPS, THETA, GROUP = 1e-5, 5e5, 128
 PROMPT, NEW_TOKENS = 1024, 128
+PAGE, KV_GROUP = 64, 64  # --kv-cache int4: tokens of a page, elements that share a scale
 
 
 def woq_weight_bytes_per_layer():
@@ -65,6 +68,20 @@ def rope(x, cos, sin):
     return torch.cat((x1 * c - x2 * s, x2 * c + x1 * s), -1)
 
 
+class Kv4Sequences:
+    """Which rows of the layers' paged 4-bit caches a call writes and attends to: `slots` and `positions` of its tokens,
+    the sequences' pages and lengths, and `starts`, the first token of every sequence (None: one token each)."""
+
+    def __init__(self, slots, positions, cos_sin, table, lens, starts=None):
+        self.slots, self.positions, self.cos_sin = slots, positions, cos_sin
+        self.table, self.lens, self.starts = table, lens, starts
+
+    def attend(self, cache, q, k, v):
+        q, k, v = (x.reshape(-1, heads, HEAD_DIM) for x, heads in ((q, HEADS), (k, KV_HEADS), (v, KV_HEADS)))
+        q = cache.append(k, v, self.slots, q, self.positions, self.cos_sin)
+        return cache.attention(q, self.table, self.lens, self.starts)
+
+
 class DecoderLayer(nn.Module):
     def __init__(self, dev):
         super().__init__()
@@ -74,11 +91,15 @@ class DecoderLayer(nn.Module):
         self.post_attention_layernorm = nn.RMSNorm(HIDDEN, eps=EPS, device=dev, dtype=torch.bfloat16)
 
     def forward(self, x, cache_k, cache_v, pos, cos, sin, mask):
-        """x [B, T, H].  pos: device int64 [T] (cache rows this call writes).  mask None = causal
+        """x [B, T, H].  With the 4-bit cache cache_k is the Kv4Sequences of the call, cache_v the layer's cache, and the
+        rest is not used.  Otherwise pos: device int64 [T] (cache rows this call writes).  mask None = causal
         prefill from an empty cache, else bool [S_max] of the cache rows a decode token may see."""
         b, t, _ = x.shape
         a = self.self_attn
         h = self.input_layernorm(x)
+        if isinstance(cache_k, Kv4Sequences):
+            o = cache_k.attend(cache_v, a.q_proj(h), a.k_proj(h), a.v_proj(h)).reshape(b, t, HEADS * HEAD_DIM)
+            return self.after_attention(x, o)
         q = a.q_proj(h).view(b, t, HEADS, HEAD_DIM).transpose(1, 2)
         k = a.k_proj(h).view(b, t, KV_HEADS, HEAD_DIM).transpose(1, 2)
         v = a.v_proj(h).view(b, t, KV_HEADS, HEAD_DIM).transpose(1, 2)
@@ -93,11 +114,13 @@ class DecoderLayer(nn.Module):
             qg = q.reshape(b, KV_HEADS, HEADS // KV_HEADS, HEAD_DIM)
             o = F.scaled_dot_product_attention(qg, cache_k, cache_v, attn_mask=mask[None, None, None, :])
             o = o.reshape(b, HEADS, 1, HEAD_DIM)
-        o = o.transpose(1, 2).reshape(b, t, HEADS * HEAD_DIM)
+        return self.after_attention(x, o.transpose(1, 2).reshape(b, t, HEADS * HEAD_DIM))
+
+    def after_attention(self, x, o):
         if hasattr(self, "mha_linear_add"):
             x = self.mha_linear_add(o, x)
         else:
-            x = x + a.o_proj(o)
+            x = x + self.self_attn.o_proj(o)
         h = self.post_attention_layernorm(x)
         if hasattr(self, "mlp_linear_add"):
             return self.mlp_linear_add(self.mlp.gate_up_fused(h), x)
@@ -163,8 +186,10 @@ def run_stack(args, peaks, clock_sampler):
     """peaks() -> (HBM GB/s, bf16 TFLOP/s, "measured" | "fallback"); clock_sampler(gpu_index) samples
     nvidia-smi while the timed regions run.  Both come from bench.py."""
     import ipex_b200
+    from ipex_b200.transformers.fusions.kv4_cache import _IPEXPagedKv4Cache
 
     ipex_b200.load_ops()
+    int4_cache = args.kv_cache == "int4"
     dev = torch.device("cuda:0")
     torch.cuda.set_device(dev)
 
@@ -179,6 +204,7 @@ def run_stack(args, peaks, clock_sampler):
     inv = 1.0 / (THETA ** (torch.arange(0, HEAD_DIM, 2, device=dev, dtype=torch.float32) / HEAD_DIM))
     ang = torch.arange(s_max, device=dev, dtype=torch.float32)[:, None] * inv[None]
     cos_t, sin_t = ang.cos().bfloat16(), ang.sin().bfloat16()
+    cos_sin = _IPEXPagedKv4Cache.rotary_table(s_max, HEAD_DIM, THETA, dev) if int4_cache else None
     hbm_peak, _, peak_kind = peaks()
     wbytes = LAYERS * woq_weight_bytes_per_layer()
     batches = [int(b) for b in str(args.stack).split(",")] if args.stack not in (None, "all") else [1, 8, 32]
@@ -188,8 +214,14 @@ def run_stack(args, peaks, clock_sampler):
     for bs in batches:
         gen = torch.Generator(device=dev).manual_seed(100 + bs)
         prompt = torch.randint(0, VOCAB, (bs, PROMPT), device=dev, generator=gen)
-        cache_k = [torch.zeros(bs, KV_HEADS, s_max, HEAD_DIM, device=dev, dtype=torch.bfloat16) for _ in layers]
-        cache_v = [torch.zeros_like(c) for c in cache_k]
+        if int4_cache:
+            pages = -(-s_max // PAGE)
+            caches = [_IPEXPagedKv4Cache(bs * pages, KV_HEADS, HEAD_DIM, PAGE, KV_GROUP, torch.bfloat16, dev) for _ in layers]
+            table = torch.arange(bs * pages, device=dev, dtype=torch.int32).view(bs, pages)
+            first_slot = torch.arange(bs, device=dev)[:, None] * (pages * PAGE)
+        else:
+            cache_k = [torch.zeros(bs, KV_HEADS, s_max, HEAD_DIM, device=dev, dtype=torch.bfloat16) for _ in layers]
+            cache_v = [torch.zeros_like(c) for c in cache_k]
 
         # ---- prefill, four sequences at a time -------------------------------------------
         tok = torch.empty(bs, dtype=torch.long, device=dev)
@@ -199,8 +231,16 @@ def run_stack(args, peaks, clock_sampler):
             for b0 in range(0, bs, 4):
                 b1 = min(bs, b0 + 4)
                 x = embed[prompt[b0:b1]]
+                n = b1 - b0
+                if int4_cache:
+                    seqs = Kv4Sequences((first_slot[b0:b1] + ppos).flatten(), ppos.repeat(n), cos_sin, table[b0:b1],
+                                        torch.full((n,), PROMPT, device=dev, dtype=torch.int32),
+                                        torch.arange(n + 1, device=dev, dtype=torch.int32) * PROMPT)
                 for i, layer in enumerate(layers):
-                    x = layer(x, cache_k[i][b0:b1], cache_v[i][b0:b1], ppos, cos_t[:PROMPT], sin_t[:PROMPT], None)
+                    if int4_cache:
+                        x = layer(x, seqs, caches[i], None, None, None, None)
+                    else:
+                        x = layer(x, cache_k[i][b0:b1], cache_v[i][b0:b1], ppos, cos_t[:PROMPT], sin_t[:PROMPT], None)
                 tok[b0:b1] = (norm(x[:, -1]) @ head.t()).argmax(-1)
 
         with torch.no_grad():
@@ -224,10 +264,16 @@ def run_stack(args, peaks, clock_sampler):
 
         def decode_step():
             x = embed[tok][:, None, :]
-            cos, sin = cos_t.index_select(0, pos), sin_t.index_select(0, pos)
-            mask = rows <= pos
+            if int4_cache:
+                seqs = Kv4Sequences((first_slot[:, 0] + pos), pos.expand(bs), cos_sin, table, (pos + 1).int().expand(bs).contiguous())
+            else:
+                cos, sin = cos_t.index_select(0, pos), sin_t.index_select(0, pos)
+                mask = rows <= pos
             for i, layer in enumerate(layers):
-                x = layer(x, cache_k[i], cache_v[i], pos, cos, sin, mask)
+                if int4_cache:
+                    x = layer(x, seqs, caches[i], None, None, None, None)
+                else:
+                    x = layer(x, cache_k[i], cache_v[i], pos, cos, sin, mask)
             nxt = (norm(x[:, 0]) @ head.t()).argmax(-1)
             tok.copy_(nxt)
             out_tokens.index_copy_(0, step_no, nxt[None])
@@ -301,15 +347,20 @@ def run_stack(args, peaks, clock_sampler):
             "distinct_tokens_generated": distinct,
         })
         log(f"stack: batch {bs}: {results[-1]}")
-        del graph, lgraph, cache_k, cache_v
+        del graph, lgraph
+        if int4_cache:
+            del caches
+        else:
+            del cache_k, cache_v
         torch.cuda.empty_cache()
     clocks = sampler.stop()
     print(json.dumps({
         "metric": "llama3_8b_int4_woq_decode_stack", "unit": "ms/token", "higher_is_better": False,
         "n_gpus": 1, "dtype": "bf16", "data": "synthetic",
         "config": {"workload": "Llama-3-8B architecture, 32 layers, INT4 asymmetric group-128 WOQ on all decoder "
-                               "linears (lm_head bf16), prompt %d, %d greedy steps, static KV cache, CUDA-graph "
-                               "decode step" % (PROMPT, new_tokens),
+                               "linears (lm_head bf16), prompt %d, %d greedy steps, %s, CUDA-graph "
+                               "decode step" % (PROMPT, new_tokens, "paged 4-bit KV cache (group %d)" % KV_GROUP if int4_cache
+                                                else "static KV cache"),
                    "woq_launches_per_token": 4 * LAYERS, "woq_weight_bytes_per_token": wbytes,
                    "inputs": "larger than L2 (%.1f GB of packed weights read per token)" % (wbytes / 1e9)},
         "roofline_peak_GBps": hbm_peak, "roofline_peak_kind": peak_kind, "results": results, "checked": True,
