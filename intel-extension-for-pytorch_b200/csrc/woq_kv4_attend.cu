@@ -23,11 +23,12 @@ constexpr int kWarps = 7;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kJoinBar = 1;
 constexpr int kMaxCtas = 512;
+constexpr int kMaxParts = 36;  // CTAs that share an item
 constexpr int kUnitKeys = 32;  // keys of a unit: two blocks
 
 // What an item costs beside its units (queries, joining the warps), in units: 222 units over 32 short sequences took
 // three times as long as over two long ones.
-constexpr int kItemCost = 24;
+constexpr int kItemCost = 18;
 
 // Two CTAs an SM where the registers allow it (their accumulators are D x 8 NT / 32 a lane), and as many ring slots as
 // fit: one SM then has up to 150 KB of copies in flight.
@@ -36,19 +37,18 @@ template <int D, int G, int NT>
 struct Smem {
   static constexpr int kCtas = ctas_per_sm(D, NT), kBlock = kv4_block_bytes(D, G);
   static constexpr size_t kBudget = kCtas == 2 ? 112 * 1024 : 226 * 1024;
-  static constexpr size_t join = 0;                              // [kWarps][kJoinD][8] sums of the values
-  static constexpr int kJoinD = kCtas == 2 || D == 64 ? 64 : 128;
-  static_assert(D % kJoinD == 0, "whole slices");
-  static constexpr size_t kJoinBytes = kWarps * kJoinD * 8 * 4;
+  static constexpr size_t join = 0;                              // [kWarps][D][8] sums of the values
+  static constexpr size_t kJoinBytes = kWarps * D * 8 * 4;
   static constexpr size_t query = join + kJoinBytes;             // [8 NT][D] of T, where registers do not hold them
   static constexpr bool kQInRegs = NT * D <= 128;
   static constexpr size_t stats = query + (kQInRegs ? 0 : 8 * NT * D * 2);  // [kWarps][8 NT]{max, sum}
   static constexpr size_t totals = stats + kWarps * 8 * NT * 8;  // [8 NT]{max, sum}
-  static constexpr size_t full = totals + 8 * NT * 8;            // [kWarps][kRing] barriers: the slot holds its block
+  static constexpr size_t row_at = totals + 8 * NT * 8;          // [8 NT] places in the output
+  static constexpr size_t full = row_at + 8 * NT * 8;            // [kWarps][kRing] barriers: the slot holds its block
   static constexpr size_t empty = full + kWarps * 8 * 8;         // the warp has read it
   static constexpr size_t left_out = empty + kWarps * 8 * 8;     // words: nothing was loaded
   static constexpr size_t ring = left_out + kWarps * 8 * 4;
-  static constexpr int kFit = static_cast<int>((kBudget - ring) / (kWarps * kBlock)), kRing = kFit >= 8 ? 8 : kFit / 2 * 2;
+  static constexpr int kFit = static_cast<int>((kBudget - ring) / (kWarps * kBlock)), kRing = kFit >= 8 ? 8 : kFit;
   static constexpr size_t total = ring + static_cast<size_t>(kWarps) * kRing * kBlock;
 };
 
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
   float* join = reinterpret_cast<float*>(smem + S::join);
   float2* stats = reinterpret_cast<float2*>(smem + S::stats);
   float2* totals = reinterpret_cast<float2*>(smem + S::totals);
+  int64_t* row_at = reinterpret_cast<int64_t*>(smem + S::row_at);
   uint16_t* qs = reinterpret_cast<uint16_t*>(smem + S::query);
 
   if (threadIdx.x < kWarps * kRing) {
@@ -151,14 +152,20 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
     const int2 chunk0 = sequence_items<kRows>(p, lane);
     auto chunk = [&](int b0) { return b0 == 0 ? chunk0 : sequence_items<kRows>(p, b0 + lane); };
     int64_t total = 0;
+    int longest = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       const int2 c = chunk(b0);
       int64_t u = static_cast<int64_t>(c.x) * (c.y + kItemCost);
+      if (c.x > 0) longest = max(longest, c.y);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+      for (int o = 16; o > 0; o >>= 1) {
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+        longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+      }
       total += u;
     }
-    const int64_t share = max(int64_t(kWarps), (total + gridDim.x - 1) / gridDim.x);
+    // (few long items: as many parts as are joined in less time than they save)
+    const int64_t share = max(max(int64_t(kWarps), (total + gridDim.x - 1) / gridDim.x), int64_t(longest / (kMaxParts - 2) + 1));
     const int64_t begin = share * blockIdx.x, end = min(total, begin + share);
     int64_t units = 0;
     if (begin < total) {
@@ -179,8 +186,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
         // units before a place in the lane's sequence
         const int64_t start = before + cost_end - cost, start_units = before_units + u_end - u;
         const int length = c.y + kItemCost;
+        auto item_of = [&](int64_t place) -> int64_t {  // (a 64-bit division takes a hundred instructions)
+          const int64_t x = place - start;
+          return x >> 32 ? x / length : static_cast<uint32_t>(x) / static_cast<uint32_t>(length);
+        };
         auto units_before = [&](int64_t place) {
-          const int64_t item = (place - start) / length;
+          const int64_t item = item_of(place);
           return start_units + item * c.y + max(int64_t(0), place - start - item * length - kItemCost);
         };
         if (!first) {
@@ -189,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
             first = true;
             const int src = __ffs(hit) - 1;
             if (lane == src) {
-              const int64_t item = (begin - start) / length;
+              const int64_t item = item_of(begin);
               first_unit = units_before(begin);
               s_b = b0 + lane;
               s_item = start + item * length;
@@ -347,11 +358,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
     // the warp's units of the item: those with (unit % kWarps) == warp
     for (int u = done + (warp - done % kWarps + kWarps) % kWarps; u < done + n; u += kWarps) {
       const int key0 = (cc.blk + u - done) * kUnitKeys;
-      const int slot0 = warp * kRing + at % kRing, use = (at / kRing) & 1;  // the unit's other block is in the next slot
+      const int slot0 = warp * kRing + at % kRing, slot1 = warp * kRing + (at + 1) % kRing;  // of the unit's two blocks
+      mbar_wait(full + slot0, (at / kRing) & 1, &s_abort, p.status, 910);
+      mbar_wait(full + slot1, ((at + 1) / kRing) & 1, &s_abort, p.status, 910);
       at += 2;
-      mbar_wait(full + slot0, use, &s_abort, p.status, 910);
-      mbar_wait(full + slot0 + 1, use, &s_abort, p.status, 910);
-      const bool have0 = !left_out[slot0], have1 = !left_out[slot0 + 1];
+      const bool have0 = !left_out[slot0], have1 = !left_out[slot1];
       // ---- scores: s[i][nt] = keys g, g + 8 of block i and rows 2 t, 2 t + 1.  Both blocks side by side: their
       // products do not wait for one another ----
       float s[2][NT][4];
@@ -367,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
         uint32_t kw[2][2][nw], wp[2][2][kGroups];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint8_t* blk = ring + (slot0 + i) * kBlock;
+          const uint8_t* blk = ring + (i ? slot1 : slot0) * kBlock;
           load_words(blk + g * (D / 2) + hh * 64 + t * nw * 4, kw[i][0]);
           load_words(blk + (g + 8) * (D / 2) + hh * 64 + t * nw * 4, kw[i][1]);
           load_words(blk + kv4_key_params(D) + (g * ng + hh * kGroups) * 4, wp[i][0]);
@@ -449,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (!(i ? have1 : have0)) continue;
-        const uint8_t* blk = ring + (slot0 + i) * kBlock;
+        const uint8_t* blk = ring + (i ? slot1 : slot0) * kBlock;
         const int left = cc.len - key0 - i * 16;  // tokens behind the last one hold anything
 #pragma unroll
         for (int hh = 0; hh < kHalves; ++hh) {
@@ -490,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
         }
       }
       __syncwarp();
-      if (lane < 2) mbar_arrive(empty + slot0 + lane);
+      if (lane < 2) mbar_arrive(empty + (lane ? slot1 : slot0));
     }
 
     // ---- the next item's queries are on their way while the warps are joined ----
@@ -506,137 +517,144 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
     constexpr int kPartial = kRows * (D + 2);
     const int64_t item_units = item_at + kItemCost;
     float* part = p.partials + (static_cast<int64_t>(blockIdx.x) * 2 + (item_units < begin ? 0 : 1)) * kPartial;
-    auto store = [&](int row, int d, float sum_pv, float sum_p) {
-      const int i = cc.r * kRows + row;
-      if (i >= cc.rows_tok * p.heads) return;
-      const int token = p.starts ? i / p.heads : 0;
-      p.out[static_cast<int64_t>(cc.q0 + token) * p.o_tok + static_cast<int64_t>(cc.h * p.heads + i - token * p.heads) * p.o_head +
-            d] = T::from_float(sum_p == 0.f ? 0.f : sum_pv / sum_p * Dequant<T>::kBack);
-    };
-    constexpr int kJoinD = S::kJoinD;
-#pragma unroll
-    for (int step = 0; step < NT * D / kJoinD; ++step) {
-      const int nt = step / (D / kJoinD), d0 = step % (D / kJoinD) * kJoinD;
-      named_bar_sync(kJoinBar, kWarps * 32);  // (what was joined before is read)
-      if (d0 == 0) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float l = sum[nt][e];
-          l += __shfl_xor_sync(0xffffffffu, l, 4);
-          l += __shfl_xor_sync(0xffffffffu, l, 8);
-          l += __shfl_xor_sync(0xffffffffu, l, 16);
-          if (g == 0) stats[warp * 8 + 2 * t + e] = make_float2(top[nt][e], l);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kJoinD / 16; ++i) {
-        const float* x = o[nt][d0 / 16 + i];
-        float* dst = join + (warp * kJoinD + 16 * i + g) * 8 + 2 * t;
-        *reinterpret_cast<float2*>(dst) = make_float2(x[0], x[1]);
-        *reinterpret_cast<float2*>(dst + 64) = make_float2(x[2], x[3]);
-      }
-      named_bar_sync(kJoinBar, kWarps * 32);
-      // a thread has rows 4 (tid & 1) .. + 3 of elements tid / 2, + 112, ..
-      const int row0 = (threadIdx.x & 1) * 4;
-      float f[kWarps][4], m[4], l[4];
+    auto store = [&](int row0, int d, const float4& v) {
+      const float r[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        m[e] = -INFINITY;
-        l[e] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) m[e] = fmaxf(m[e], stats[w * 8 + row0 + e].x);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 st = stats[w * 8 + row0 + e];
-          // (a warp without a score has sums of zero, or of NaN)
-          f[w][e] = st.x == -INFINITY ? 1.f : exp2_approx(st.x - m[e]);
-          l[e] = fmaf(st.y, f[w][e], l[e]);
-        }
+        const int64_t at = row_at[row0 + e];
+        const float l = totals[row0 + e].y;
+        if (at >= 0) p.out[at + d] = T::from_float(l == 0.f ? 0.f : __fdividef(r[e], l) * Dequant<T>::kBack);
       }
-      for (int i = threadIdx.x; i < kJoinD * 2; i += kWarps * 32) {
-        const int d = d0 + i / 2;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
+    };
+    // eight rows at a time: every warp's sums against the rows' common maximum, added in the order of the warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = sum[nt][e];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        if (g == 0) stats[warp * 8 + 2 * t + e] = make_float2(top[nt][e], l);
+      }
+      named_bar_sync(kJoinBar, kWarps * 32);  // (what was joined before is read, too)
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, stats[w * 8 + 2 * t + e].x);
+        // (a warp without a score has sums of zero, or of NaN)
+        f[e] = top[nt][e] == -INFINITY ? 1.f : exp2_approx(top[nt][e] - m);
+      }
+#pragma unroll
+      for (int i = 0; i < kMt; ++i) {
+        const float* x = o[nt][i];
+        float* dst = join + (warp * D + 16 * i + g) * 8 + 2 * t;
+        *reinterpret_cast<float2*>(dst) = make_float2(x[0] * f[0], x[1] * f[1]);
+        *reinterpret_cast<float2*>(dst + 64) = make_float2(x[2] * f[0], x[3] * f[1]);
+      }
+      // (where rows go is looked up once: the code of a small call runs from a cold instruction cache)
+      if (nt == 0 && threadIdx.x < kRows) {
+        const int i = cc.r * kRows + threadIdx.x, token = p.starts ? i / p.heads : 0;
+        row_at[threadIdx.x] = i < cc.rows_tok * p.heads ? static_cast<int64_t>(cc.q0 + token) * p.o_tok +
+                                                            static_cast<int64_t>(cc.h * p.heads + i - token * p.heads) * p.o_head
+                                                      : -1;
+      }
+      if (threadIdx.x < 8) {
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, stats[w * 8 + threadIdx.x].x);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(join + w * kJoinD * 8 + i * 4);
-          v[0] = fmaf(x.x, f[w][0], v[0]);
-          v[1] = fmaf(x.y, f[w][1], v[1]);
-          v[2] = fmaf(x.z, f[w][2], v[2]);
-          v[3] = fmaf(x.w, f[w][3], v[3]);
+          const float2 st = stats[w * 8 + threadIdx.x];
+          l = fmaf(st.y, st.x == -INFINITY ? 1.f : exp2_approx(st.x - m), l);
+        }
+        totals[nt * 8 + threadIdx.x] = make_float2(m, l);
+        if (!whole) *reinterpret_cast<float2*>(part + 2 * (nt * 8 + threadIdx.x)) = make_float2(m, l);
+      }
+      named_bar_sync(kJoinBar, kWarps * 32);
+      for (int i = threadIdx.x; i < D * 2; i += kWarps * 32) {  // element i / 2, four rows
+        const int d = i / 2, row0 = (i & 1) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 x = *reinterpret_cast<const float4*>(join + w * D * 8 + i * 4);
+          v.x += x.x;
+          v.y += x.y;
+          v.z += x.z;
+          v.w += x.w;
         }
         if (whole) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) store(nt * 8 + row0 + e, d, v[e], l[e]);
+          store(nt * 8 + row0, d, v);
         } else {
-          *reinterpret_cast<float4*>(part + 2 * kRows + d * kRows + nt * 8 + row0) = make_float4(v[0], v[1], v[2], v[3]);
-          if (d == 0) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(part + 2 * (nt * 8 + row0 + e)) = make_float2(m[e], l[e]);
-          }
+          *reinterpret_cast<float4*>(part + 2 * kRows + d * kRows + nt * 8 + row0) = v;
         }
       }
+      if (nt + 1 < NT) named_bar_sync(kJoinBar, kWarps * 32);  // (the statistics' place is written again)
     }
     if (!whole) {
       // ---- the last CTA of the item joins the parts ----
       const int first = static_cast<int>(item_units / share);
       const int parts = static_cast<int>((item_units + cc.blocks - 1) / share) - first + 1;
-      __threadfence();
       named_bar_sync(kJoinBar, kWarps * 32);
       if (threadIdx.x == 0) {
+        __threadfence();
         const uint32_t before = atomicAdd(p.counters + first, 1u);
         s_last = before == static_cast<uint32_t>(parts - 1);
         if (s_last) p.counters[first] = 0;
+        __threadfence();
       }
       named_bar_sync(kJoinBar, kWarps * 32);
       if (s_last) {
-        __threadfence();
-        auto part_of = [&](int c) {
-          return p.partials + (static_cast<int64_t>(first + c) * 2 + (item_units < (first + c) * share ? 0 : 1)) * kPartial;
-        };
-        // weights of the parts, [part][row] for as many parts at a time as the joining buffer takes
-        float* wt = join;
-        constexpr int kChunk = static_cast<int>(S::kJoinBytes) / (kRows * 4), kQuads = (D * 2 * NT + kWarps * 32 - 1) / (kWarps * 32);
-        float mm = -INFINITY, l = 0.f;
-        if (threadIdx.x < kRows)
-          for (int c = 0; c < parts; ++c) mm = fmaxf(mm, __ldcg(part_of(c) + 2 * threadIdx.x));
-        float4 v[kQuads];
+        // Statistics of all parts at once, eight lanes a row weigh them, then the sums in the order of the parts, four in
+        // flight.  Small code: it runs once, from a cold instruction cache.
+        // (the item begins in its first CTA's share and before all others')
+        auto part_of = [&](int c) { return p.partials + (2 * (first + c) + (c == 0)) * kPartial; };
+        float2* ps = reinterpret_cast<float2*>(join);               // [part][row]
+        float* weight = join + 2 * kMaxParts * kRows;               // [part][row]
+        static_assert(3 * kMaxParts * kRows * 4 <= S::kJoinBytes, "joining buffer");
+        for (int i = threadIdx.x; i < parts * kRows; i += kWarps * 32)
+          ps[i] = __ldcg(reinterpret_cast<const float2*>(part_of(i / kRows)) + i % kRows);
+        named_bar_sync(kJoinBar, kWarps * 32);
+        for (int row = threadIdx.x >> 3; row < kRows; row += kWarps * 4) {  // (four rows a warp: it stays together)
+          const int sub = threadIdx.x & 7;
+          float m = -INFINITY, l = 0.f;
+          for (int c = sub; c < parts; c += 8) m = fmaxf(m, ps[c * kRows + row].x);
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          for (int c = sub; c < parts; c += 8) {
+            const float2 st = ps[c * kRows + row];
+            const float f = st.x == -INFINITY ? 1.f : exp2_approx(st.x - m);  // (nothing seen: sums of zero, or of NaN)
+            weight[c * kRows + row] = f;
+            l = fmaf(st.y, f, l);
+          }
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          if (sub == 0) totals[row] = make_float2(m, l);
+        }
+        named_bar_sync(kJoinBar, kWarps * 32);
+        for (int i = threadIdx.x; i < D * 2 * NT; i += kWarps * 32) {
+          const int d = i / (2 * NT), row0 = i % (2 * NT) * 4;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c0 = 0; c0 < parts; c0 += 4) {
+            float4 x[4];
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c0 = 0; c0 < parts; c0 += kChunk) {
-          const int c1 = min(parts, c0 + kChunk);
-          if (c0) named_bar_sync(kJoinBar, kWarps * 32);
-          if (threadIdx.x < kRows)
-            for (int c = c0; c < c1; ++c) {
-              const float2 st = __ldcg(reinterpret_cast<const float2*>(part_of(c) + 2 * threadIdx.x));
-              const float f = st.x == -INFINITY ? 0.f : exp2_approx(st.x - mm);
-              wt[(c - c0) * kRows + threadIdx.x] = f;
-              l += st.x == -INFINITY ? st.y : st.y * f;
-            }
-          named_bar_sync(kJoinBar, kWarps * 32);
+            for (int k = 0; k < 4; ++k)
+              x[k] = __ldcg(reinterpret_cast<const float4*>(part_of(min(c0 + k, parts - 1)) + 2 * kRows) + i);
 #pragma unroll
-          for (int i = 0; i < kQuads; ++i) {
-            const int at = threadIdx.x + i * kWarps * 32;
-            if (at >= D * 2 * NT) break;
-            for (int c = c0; c < c1; ++c) {
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(part_of(c) + 2 * kRows + at * 4));
-              const float4 f = *reinterpret_cast<const float4*>(wt + (c - c0) * kRows + at % (2 * NT) * 4);
-              v[i].x = fmaf(x.x, f.x, v[i].x);
-              v[i].y = fmaf(x.y, f.y, v[i].y);
-              v[i].z = fmaf(x.z, f.z, v[i].z);
-              v[i].w = fmaf(x.w, f.w, v[i].w);
+            for (int k = 0; k < 4; ++k) {
+              if (c0 + k >= parts) break;
+              const float4 f = *reinterpret_cast<const float4*>(weight + (c0 + k) * kRows + row0);
+              v.x = fmaf(x[k].x, f.x, v.x);
+              v.y = fmaf(x[k].y, f.y, v.y);
+              v.z = fmaf(x[k].z, f.z, v.z);
+              v.w = fmaf(x[k].w, f.w, v.w);
             }
           }
-        }
-        if (threadIdx.x < kRows) totals[threadIdx.x] = make_float2(mm, l);
-        named_bar_sync(kJoinBar, kWarps * 32);
-#pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-          const int quad = threadIdx.x + i * kWarps * 32;
-          if (quad >= D * 2 * NT) break;
-          const int d = quad / (2 * NT), row0 = quad % (2 * NT) * 4;
-          const float r[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) store(row0 + e, d, r[e], totals[row0 + e].y);
+          store(row0, d, v);
         }
       }
     }
