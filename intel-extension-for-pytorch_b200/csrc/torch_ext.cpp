@@ -14,6 +14,7 @@
 #include <ATen/ATen.h>
 #include <ATen/autocast_mode.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -552,26 +553,30 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> woq_add_rmsnorm_quant
   TORCH_CHECK(input.dim() >= 1, "WOQ: add_rmsnorm_quant takes rows");
   const int64_t K = input.size(-1);
   TORCH_CHECK(weight.numel() == K, "WOQ: the norm weight has ", weight.numel(), " elements, expected ", K);
-  c10::cuda::CUDAGuard guard(input.device());
+  const c10::DeviceIndex dev = input.get_device();
+  c10::cuda::CUDAGuard guard(dev);
+  // (a decode step makes this call for a kernel of three microseconds: nothing is dispatched that need not be)
+  auto aligned = [](const at::Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; };
   auto rows = [&](const at::Tensor& t) {
-    at::Tensor x = t.reshape({-1, K});
-    if (x.stride(-1) != 1 || x.stride(0) < K || (x.stride(0) % 8) != 0 || (reinterpret_cast<uintptr_t>(x.data_ptr()) & 15))
-      x = x.contiguous();
-    return x;
+    at::Tensor x = t.dim() == 2 ? t : t.reshape({-1, K});
+    return x.stride(1) == 1 && x.stride(0) >= K && x.stride(0) % 8 == 0 && aligned(x) ? x : x.clone(at::MemoryFormat::Contiguous);
   };
   const at::Tensor x = rows(input), r = rows(residual);
-  at::Tensor g = weight.to(input.device(), at::kBFloat16).contiguous();
-  if (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15) g = g.clone();
+  at::Tensor g = weight;
+  if (g.get_device() != dev || !g.is_cuda() || g.scalar_type() != at::kBFloat16 || !g.is_contiguous())
+    g = g.to(input.device(), at::kBFloat16).contiguous();
+  if (!aligned(g)) g = g.clone();
   const int64_t M = x.size(0);
-  at::Tensor sum = at::empty(input.sizes(), x.options());
-  at::Tensor qa = at::empty(input.sizes(), x.options().dtype(at::kChar));
-  at::Tensor sa = at::empty({M}, x.options().dtype(at::kFloat));
   const bool asym = act_quant_mode == WOQ_B200_ACT_PER_M;
-  at::Tensor zpa = at::empty({asym ? M : 0}, x.options().dtype(at::kInt));
-  auto stream = at::cuda::getCurrentCUDAStream(input.get_device());
+  auto make = [&](at::IntArrayRef sizes, at::ScalarType type) {
+    return at::detail::empty_cuda(sizes, type, input.device(), c10::nullopt);
+  };
+  at::Tensor sum = make(input.sizes(), at::kBFloat16), qa = make(input.sizes(), at::kChar), sa = make({M}, at::kFloat);
+  at::Tensor zpa = make({asym ? M : 0}, at::kInt);
   WOQ_CHECK(woq_b200_add_rmsnorm_quant(x.data_ptr(), x.stride(0), r.data_ptr(), r.stride(0), g.data_ptr(),
                                        static_cast<float>(eps), M, K, static_cast<int32_t>(act_quant_mode), sum.data_ptr(),
-                                       K, qa.data_ptr(), sa.data_ptr(), asym ? zpa.data_ptr() : nullptr, stream.stream()));
+                                       K, qa.data_ptr(), sa.data_ptr(), asym ? zpa.data_ptr() : nullptr,
+                                       at::cuda::getCurrentCUDAStream(dev).stream()));
   return std::make_tuple(sum, qa, sa, zpa);
 }
 
@@ -607,7 +612,11 @@ at::Tensor kv4_rows(const at::Tensor& t, const at::Tensor& cache, at::ScalarType
 at::Tensor kv4_index(const at::Tensor& t, const at::Tensor& cache, at::ScalarType dtype, const char* what) {
   TORCH_CHECK(t.device() == cache.device() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong), "WOQ: ", what,
               " must be a tensor of int32 or int64 on the cache's device");
+  if (t.scalar_type() == dtype && t.is_contiguous()) return t;
   return t.to(dtype).contiguous();
+}
+at::Tensor kv4_empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& cache) {
+  return at::detail::empty_cuda(sizes, type, cache.device(), c10::nullopt);
 }
 
 at::Tensor kv4_cache_append(at::Tensor& cache, const at::Tensor& key, const at::Tensor& value, const at::Tensor& slots,
@@ -628,9 +637,9 @@ at::Tensor kv4_cache_append(at::Tensor& cache, const at::Tensor& key, const at::
     q = kv4_rows(*query, cache, dtype, "query");
     TORCH_CHECK(q.size(0) == tokens && q.size(2) == key.size(2), "WOQ: query must be [tokens, q heads, head_dim]");
     TORCH_CHECK(q.size(1) >= 1 && q.size(1) <= 65535, "WOQ: the number of query heads is out of range");
-    q_out = at::empty(q.sizes(), key.options());
+    q_out = kv4_empty(q.sizes(), dtype, cache);
   } else {
-    q_out = at::empty({0}, key.options());
+    q_out = kv4_empty({0}, dtype, cache);
   }
   int64_t rot = 0;
   const bool turns = cos_sin.has_value() && cos_sin->defined();
@@ -661,7 +670,7 @@ std::tuple<at::Tensor, at::Tensor> kv4_cache_read(const at::Tensor& cache, const
   c10::cuda::CUDAGuard guard(cache.device());
   const at::Tensor s = kv4_index(slots, cache, at::kLong, "slots");
   TORCH_CHECK(s.dim() == 1, "WOQ: slots must be one-dimensional");
-  at::Tensor k = at::empty({s.size(0), d.kv_heads, head_dim}, cache.options().dtype(dtype)), v = at::empty_like(k);
+  at::Tensor k = kv4_empty({s.size(0), d.kv_heads, head_dim}, dtype, cache), v = kv4_empty(k.sizes(), dtype, cache);
   WOQ_CHECK(woq_b200_kv4_read(&d, cache.data_ptr(), s.data_ptr<int64_t>(), s.size(0), k.data_ptr(), v.data_ptr(),
                               at::cuda::getCurrentCUDAStream(cache.get_device()).stream()));
   return std::make_tuple(k, v);
@@ -689,7 +698,7 @@ at::Tensor kv4_cache_attention(const at::Tensor& query, const at::Tensor& cache,
                 batch, " sequences");
   }
   // (rows that belong to no sequence are zeros)
-  at::Tensor out = starts.defined() ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());
+  at::Tensor out = starts.defined() ? at::zeros(q.sizes(), q.options()) : kv4_empty(q.sizes(), q.scalar_type(), cache);
   if (batch == 0 || tokens == 0) return out;
   auto stream = at::cuda::getCurrentCUDAStream(cache.get_device());
   const size_t need = woq_b200_kv4_attention_workspace_bytes(&d, batch, tokens, static_cast<int32_t>(heads));

@@ -434,9 +434,10 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
     const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(h[i][j] << 16) * inv * __uint_as_float(gw[j] << 16),
-                                                     __uint_as_float(h[i][j] & 0xffff0000u) * inv *
-                                                         __uint_as_float(gw[j] & 0xffff0000u));
+      // (the product of two bf16 numbers is exact: one rounding in 32 bits less than h * inv * g)
+      const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(h[i][j] << 16) * __uint_as_float(gw[j] << 16) * inv,
+                                                     __uint_as_float(h[i][j] & 0xffff0000u) *
+                                                         __uint_as_float(gw[j] & 0xffff0000u) * inv);
       h[i][j] = *reinterpret_cast<const uint32_t*>(&y);
       const float a = __uint_as_float(h[i][j] << 16), b = __uint_as_float(h[i][j] & 0xffff0000u);
       lo = fminf(lo, fminf(a, b));

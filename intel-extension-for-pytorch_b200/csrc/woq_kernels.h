@@ -426,10 +426,13 @@ struct Kv4AttendParams {
   int batch, tokens, q_heads, kv_heads, heads;  // heads: query heads of a kv head
   int page_blocks, max_blocks, causal;
   int page_shift;         // log2 of page_blocks, or -1 (set by the launch)
+  int splits;             // prompts: CTAs that share a tile of rows (set by the launch)
 };
 int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d);
-size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int d, int num_sms);
+size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms);
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, int num_sms, cudaStream_t stream);
+int kv4_prompt_splits(int batch, int64_t tokens, int heads, int kv_heads, int d, int64_t max_keys, int num_sms);
+size_t kv4_prompt_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms);
 cudaError_t launch_kv4_prompt(const Kv4AttendParams& p, int f16, int d, int g, cudaStream_t stream);
 constexpr int kStatusBadPage = 901;  // a block table names a page that the cache does not have
 

@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
   constexpr int ng = D / G, kGroups = ng / kHalves, kWordsPerGroup = G / 32, kMt = D / 16;
   constexpr bool kQInRegs = S::kQInRegs;
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t s_run[kThreads / 32][3];  // {cost, units, longest item} of the sequences of a warp
   __shared__ int64_t s_share, s_item;  // share of a CTA; where the first item begins (both with kItemCost an item)
   __shared__ int s_b, s_in_b, s_units, s_last;
   __shared__ volatile int s_abort;
@@ -147,77 +148,97 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
   grid_launch_dependents();
   grid_dependency_wait();
 
-  // ---- this CTA's share: [begin, end) of all items' units, every item preceded by kItemCost that nobody computes ----
-  if (warp == 0) {
-    const int2 chunk0 = sequence_items<kRows>(p, lane);
-    auto chunk = [&](int b0) { return b0 == 0 ? chunk0 : sequence_items<kRows>(p, b0 + lane); };
-    int64_t total = 0;
+  // ---- this CTA's share: [begin, end) of all items' units, every item preceded by kItemCost that nobody computes.  Every
+  // warp adds up a run of the sequences (their lengths all on their way at once), the first one looks into two of the
+  // runs for the ends of the share ----
+  const int run = (p.batch + kThreads - 1) / kThreads * 32;  // sequences of a warp
+  {
+    int64_t cost = 0, u = 0;
     int longest = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      const int2 c = chunk(b0);
-      int64_t u = static_cast<int64_t>(c.x) * (c.y + kItemCost);
+#pragma unroll 4
+    for (int b = warp * run + lane; b < min(p.batch, (warp + 1) * run); b += 32) {
+      const int2 c = sequence_items<kRows>(p, b);
+      cost += static_cast<int64_t>(c.x) * (c.y + kItemCost);
+      u += static_cast<int64_t>(c.x) * c.y;
       if (c.x > 0) longest = max(longest, c.y);
+    }
+    if (warp * run < p.batch) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
+        cost += __shfl_xor_sync(0xffffffffu, cost, o);
         u += __shfl_xor_sync(0xffffffffu, u, o);
         longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
       }
-      total += u;
+    }
+    if (lane == 0) {
+      s_run[warp][0] = cost;
+      s_run[warp][1] = u;
+      s_run[warp][2] = longest;
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int64_t total = 0, longest = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      total += s_run[w][0];
+      longest = max(longest, s_run[w][2]);
     }
     // (few long items: as many parts as are joined in less time than they save)
-    const int64_t share = max(max(int64_t(kWarps), (total + gridDim.x - 1) / gridDim.x), int64_t(longest / (kMaxParts - 2) + 1));
+    const int64_t share = max(max(int64_t(kWarps), (total + gridDim.x - 1) / gridDim.x), longest / (kMaxParts - 2) + 1);
     const int64_t begin = share * blockIdx.x, end = min(total, begin + share);
     int64_t units = 0;
     if (begin < total) {
-      int64_t before = 0, before_units = 0, first_unit = 0;  // of the sequences before b0
-      bool first = false;
-      for (int b0 = 0;; b0 += 32) {
-        const int2 c = chunk(b0);
-        const int64_t cost = static_cast<int64_t>(c.x) * (c.y + kItemCost), u = static_cast<int64_t>(c.x) * c.y;
-        int64_t cost_end = cost, u_end = u;
+      // the units before `place` of the sequence of all items; the sequence, item within it and its beginning
+      auto locate = [&](int64_t place, int64_t& item_begin, int& b_out, int& item_out) -> int64_t {
+        int64_t before = 0, before_units = 0;  // of the sequences before b0
+        int b0 = 0;
+        for (int w = 0; w + 1 < kThreads / 32 && before + s_run[w][0] <= place; ++w) {
+          before += s_run[w][0];
+          before_units += s_run[w][1];
+          b0 += run;
+        }
+        for (;; b0 += 32) {
+          const int2 c = sequence_items<kRows>(p, b0 + lane);
+          const int64_t cost = static_cast<int64_t>(c.x) * (c.y + kItemCost), u = static_cast<int64_t>(c.x) * c.y;
+          int64_t cost_end = cost, u_end = u;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t x = __shfl_up_sync(0xffffffffu, cost_end, o), y = __shfl_up_sync(0xffffffffu, u_end, o);
-          if (lane >= o) {
-            cost_end += x;
-            u_end += y;
-          }
-        }
-        // units before a place in the lane's sequence
-        const int64_t start = before + cost_end - cost, start_units = before_units + u_end - u;
-        const int length = c.y + kItemCost;
-        auto item_of = [&](int64_t place) -> int64_t {  // (a 64-bit division takes a hundred instructions)
-          const int64_t x = place - start;
-          return x >> 32 ? x / length : static_cast<uint32_t>(x) / static_cast<uint32_t>(length);
-        };
-        auto units_before = [&](int64_t place) {
-          const int64_t item = item_of(place);
-          return start_units + item * c.y + max(int64_t(0), place - start - item * length - kItemCost);
-        };
-        if (!first) {
-          const uint32_t hit = __ballot_sync(0xffffffffu, start + cost > begin);
-          if (hit) {
-            first = true;
-            const int src = __ffs(hit) - 1;
-            if (lane == src) {
-              const int64_t item = item_of(begin);
-              first_unit = units_before(begin);
-              s_b = b0 + lane;
-              s_item = start + item * length;
-              s_in_b = static_cast<int>(item);
+          for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, cost_end, o), y = __shfl_up_sync(0xffffffffu, u_end, o);
+            if (lane >= o) {
+              cost_end += x;
+              u_end += y;
             }
-            first_unit = __shfl_sync(0xffffffffu, first_unit, src);
           }
+          const uint32_t hit = __ballot_sync(0xffffffffu, before + cost_end > place);
+          if (hit) {
+            const int src = __ffs(hit) - 1, length = c.y + kItemCost;
+            const int64_t start = before + cost_end - cost, x = place - start;
+            // (a 64-bit division takes a hundred instructions)
+            const int64_t item = lane != src ? 0 : x >> 32 ? x / length : static_cast<uint32_t>(x) / static_cast<uint32_t>(length);
+            const int64_t at = before_units + u_end - u + item * c.y + max(int64_t(0), x - item * length - kItemCost);
+            item_begin = __shfl_sync(0xffffffffu, start + item * length, src);
+            item_out = static_cast<int>(__shfl_sync(0xffffffffu, item, src));
+            b_out = b0 + src;
+            return __shfl_sync(0xffffffffu, at, src);
+          }
+          before += __shfl_sync(0xffffffffu, cost_end, 31);
+          before_units += __shfl_sync(0xffffffffu, u_end, 31);
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, start + cost >= end);
-        if (hit) {
-          const int src = __ffs(hit) - 1;
-          units = (lane == src ? units_before(end) : 0) - first_unit;
-          units = __shfl_sync(0xffffffffu, units, src);
-          break;
-        }
-        before += __shfl_sync(0xffffffffu, cost_end, 31);
-        before_units += __shfl_sync(0xffffffffu, u_end, 31);
+      };
+      int64_t item_begin, unused;
+      int b, in_b, unused_b, unused_in;
+      units = -locate(begin, item_begin, b, in_b);
+      if (end < total) {
+        units += locate(end, unused, unused_b, unused_in);
+      } else {
+#pragma unroll
+        for (int w = 0; w < kThreads / 32; ++w) units += s_run[w][1];
+      }
+      if (lane == 0) {
+        s_b = b;
+        s_in_b = in_b;
+        s_item = item_begin;
       }
     }
     if (lane == 0) {
@@ -714,19 +735,23 @@ int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d) {
   return 4;
 }
 
-size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int d, int num_sms) {
-  const int nt = kv4_attend_tiles(batch, tokens, heads, d);
-  return static_cast<size_t>(ctas_for(nt, d, num_sms)) * 2 * 8 * nt * (d + 2) * 4;
-}
-
 // Whether the prompt kernel takes a call: its tiles have 128 rows, the ones above 8, 16 or 32.
 bool kv4_attend_prompt(int batch, int64_t tokens, int heads) { return ceil_div(tokens, batch) * heads > 32; }
+
+size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms) {
+  const int nt = kv4_attend_tiles(batch, tokens, heads, d);
+  const size_t few = static_cast<size_t>(ctas_for(nt, d, num_sms)) * 2 * 8 * nt * (d + 2) * 4;
+  return kv4_attend_prompt(batch, tokens, heads) ? std::max(few, kv4_prompt_partial_bytes(batch, tokens, heads, kv_heads, d, num_sms)) : few;
+}
 
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, int num_sms, cudaStream_t stream) {
   Kv4AttendParams q = p;
   q.page_shift = (p.page_blocks & (p.page_blocks - 1)) ? -1 : __builtin_ctz(static_cast<unsigned>(p.page_blocks));
   q.scale *= f16 ? Dequant<Kv4Fp16>::kBack : Dequant<Kv4Bf16>::kBack;
-  if (p.starts && kv4_attend_prompt(p.batch, p.tokens, p.heads)) return launch_kv4_prompt(q, f16, d, g, stream);
+  if (p.starts && kv4_attend_prompt(p.batch, p.tokens, p.heads)) {
+    q.splits = kv4_prompt_splits(p.batch, p.tokens, p.heads, p.kv_heads, d, static_cast<int64_t>(p.max_blocks) * kKv4Tokens, num_sms);
+    return launch_kv4_prompt(q, f16, d, g, stream);
+  }
   const int nt = kv4_attend_tiles(p.batch, p.tokens, p.heads, d);
   const int ctas = ctas_for(nt, d, num_sms);
 #define KV4_NT(NT) f16 ? launch_shape<Kv4Fp16, NT>(q, d, g, ctas, stream) : launch_shape<Kv4Bf16, NT>(q, d, g, ctas, stream)

@@ -141,7 +141,7 @@ size_t woq_b200_kv4_attention_workspace_bytes(const woq_b200_kv4_desc* d, int64_
   int sms = 0;
   if (num_sms(&sms) != WOQ_B200_OK) return 0;
   if (batch == 0 || tokens == 0) return partials_off();
-  return partials_off() + woq::kv4_attend_partial_bytes(static_cast<int>(batch), tokens, q_heads / d->kv_heads, d->head_dim, sms);
+  return partials_off() + woq::kv4_attend_partial_bytes(static_cast<int>(batch), tokens, q_heads / d->kv_heads, d->kv_heads, d->head_dim, sms);
 }
 
 int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const void* q, int64_t q_tok, int64_t q_head,
@@ -167,7 +167,7 @@ int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const 
   if (tokens > INT32_MAX / heads || static_cast<double>(batch) * d->kv_heads * (1.0 + max_pages * (d->page_size / 16.0)) *
                                             (1.0 + static_cast<double>(tokens) * heads / 8) > 1e12)
     return set_error(WOQ_B200_ERR_UNSUPPORTED, "too many query rows and cached tokens for one call");
-  if (!seq_lens || !block_table || !workspace || (d->num_pages > 0 && !cache))
+  if (!seq_lens || (max_pages > 0 && !block_table) || !workspace || (d->num_pages > 0 && !cache))
     return set_error(WOQ_B200_ERR_INVALID_ARG, "cache, block_table, seq_lens and workspace must be non-null");
   if (!aligned16(cache) || !aligned16(workspace))
     return set_error(WOQ_B200_ERR_INVALID_ARG, "cache and workspace must be 16-byte aligned");
@@ -176,7 +176,7 @@ int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const 
   if (int rc = check_rows("out", out, o_tok, o_head)) return rc;
   int sms = 0;
   if (int rc = num_sms(&sms)) return rc;
-  const size_t need = partials_off() + woq::kv4_attend_partial_bytes(static_cast<int>(batch), tokens, heads, d->head_dim, sms);
+  const size_t need = partials_off() + woq::kv4_attend_partial_bytes(static_cast<int>(batch), tokens, heads, d->kv_heads, d->head_dim, sms);
   if (workspace_bytes < need)
     return set_error(WOQ_B200_ERR_WORKSPACE, "workspace has %zu bytes, need %zu", workspace_bytes, need);
   uint8_t* ws = static_cast<uint8_t*>(workspace);

@@ -11,6 +11,8 @@
 // registers, one tile ahead; the dequantised values (bf16: times 2^-64, see Dequant) never leave the SM.
 // The running reference of the maximum is raised only when a score passes it by 8 (log2): P is at most 256 and O is
 // rescaled seldom.
+#include <algorithm>
+
 #include "woq_kernels.h"
 #include "woq_kv4_common.cuh"
 #include "woq_kv4_dequant.cuh"
@@ -39,6 +41,7 @@ struct Header {
   uint32_t tmem;
   int abort_flag;
   int bad_page;  // a page of the sequence does not exist
+  int last[2];   // this CTA joins the parts of the tile of rows
   int b, tile;
 };
 static_assert(sizeof(Header) <= 1024, "header");
@@ -248,10 +251,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
   }
   grid_launch_dependents();
   grid_dependency_wait();
-  const int h = blockIdx.x % p.kv_heads;
+  const int part = blockIdx.x % p.splits, item = blockIdx.x / p.splits, h = item % p.kv_heads;
   if (warp == 0) {
     int b, tile;
-    find_tile<kRows>(p, blockIdx.x / p.kv_heads, b, tile);
+    find_tile<kRows>(p, item / p.kv_heads, b, tile);
     if (lane == 0) {
       hd->b = b;
       hd->tile = tile;
@@ -275,6 +278,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       if (last < row_base + i * 128) limit = 0;       // no rows
       tiles_of[i] = (max(0, min(limit, len)) + KT - 1) / KT;
       n_max = max(n_max, tiles_of[i]);
+    }
+    // with few tiles of rows several CTAs share one: each takes a run of the tiles of keys, from tile `first`
+    const int first = p.splits > 1 ? static_cast<int>(static_cast<int64_t>(n_max) * part / p.splits) : 0;
+    if (p.splits > 1) {
+      const int end = static_cast<int>(static_cast<int64_t>(n_max) * (part + 1) / p.splits);
+      n_max = end - first;
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) tiles_of[i] = max(0, min(tiles_of[i], end) - first);
     }
     const int32_t* table = p.table + static_cast<int64_t>(b) * p.table_ld;
 
@@ -320,7 +331,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
       for (int j = 0; j < n; ++j) {
-        const int key0 = j * KT;
+        const int key0 = (first + j) * KT;
         mbar_wait(&hd->s_full[i], j & 1, abort_flag, p.status, 920);
         tc_fence_after_sync();
         uint32_t gone = 0;  // blocks of the tile whose page does not exist: masked (looked up if the sequence has any)
@@ -362,17 +373,76 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         mbar_arrive(&hd->p_full[i]);
       }
       // ---- the rows' results ----
+      bool last = true;
       if (n > 0) {
         mbar_wait(&hd->o_full[i], (n - 1) & 1, abort_flag, p.status, 922);
         tc_fence_after_sync();
       }
+      // Parts of a row: {maximum, sum}, then its sums of values, four at a time, a row next to the other.  The last CTA adds
+      // them in the order of the keys.
+      constexpr int kPart = 128 * (D + 2);
+      const float* parts = p.partials + (static_cast<int64_t>(item) * NQ + i) * p.splits * kPart;
+      if (p.splits > 1) {
+        const int r = quarter * 32 + lane;
+        float* mine = p.partials + ((static_cast<int64_t>(item) * NQ + i) * p.splits + part) * kPart;
+        *reinterpret_cast<float2*>(mine + 2 * r) = make_float2(top, sum);
+#pragma unroll 1
+        for (int c = 0; c < D / 32 && n > 0; ++c) {
+          uint32_t x[32];
+          tmem_ld_x32(t_o + c * 32, x);
+          wait_ld_x32(x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<uint4*>(mine + 256 + (c * 8 + e) * 512 + r * 4) = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+        }
+        named_bar_sync(1 + i, 128);
+        if (quarter == 0 && lane == 0) {
+          __threadfence();
+          const uint32_t before = atomicAdd(p.counters + item * NQ + i, 1u);
+          hd->last[i] = before == static_cast<uint32_t>(p.splits - 1);
+          if (hd->last[i]) p.counters[item * NQ + i] = 0;
+          __threadfence();
+        }
+        named_bar_sync(1 + i, 128);
+        last = hd->last[i];
+        if (last) {
+          top = -INFINITY;
+          sum = 0.f;
+#pragma unroll 1
+          for (int k = 0; k < p.splits; ++k) top = fmaxf(top, __ldcg(parts + k * kPart + 2 * r));
+#pragma unroll 1
+          for (int k = 0; k < p.splits; ++k) {
+            const float2 st = __ldcg(reinterpret_cast<const float2*>(parts + k * kPart + 2 * r));
+            sum = fmaf(st.y, st.x == -INFINITY ? 1.f : exp2_approx(st.x - top), sum);
+          }
+        }
+      }
       const float inv = sum == 0.f ? 0.f : Dequant<T>::kBack / sum;
+      if (last) {
       // to the place of the warp's query rows (their products are done) and from there, a row by D / 8 lanes
       uint8_t* stage = smem + S::q + i * S::kQBytes + quarter * 32 * 128;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t r[32];
-        if (n > 0) {
+        if (p.splits > 1) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) r[e] = 0u;
+#pragma unroll 1
+          for (int k = 0; k < p.splits; ++k) {
+            const float* from = parts + k * kPart;
+            const int rr = quarter * 32 + lane;
+            const float2 st = __ldcg(reinterpret_cast<const float2*>(from + 2 * rr));
+            if (st.x == -INFINITY && st.y == 0.f) continue;  // saw nothing: its sums were not written
+            const float f = st.x == -INFINITY ? 1.f : exp2_approx(st.x - top);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(from + 256 + (c * 8 + e) * 512 + rr * 4));
+              const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int q = 0; q < 4; ++q) r[4 * e + q] = __float_as_uint(fmaf(xs[q], f, __uint_as_float(r[4 * e + q])));
+            }
+          }
+        } else if (n > 0) {
           tmem_ld_x32(t_o + c * 32, r);
           wait_ld_x32(r);
         }
@@ -381,7 +451,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            w[k] = n > 0 && sum != 0.f ? T::pack(__uint_as_float(r[e * 8 + k * 2]) * inv, __uint_as_float(r[e * 8 + k * 2 + 1]) * inv) : 0u;
+            w[k] = sum != 0.f ? T::pack(__uint_as_float(r[e * 8 + k * 2]) * inv, __uint_as_float(r[e * 8 + k * 2 + 1]) * inv) : 0u;
           const int ch = c * 4 + e;
           *reinterpret_cast<uint4*>(stage + (ch >> 3) * (128 * 128) + lane * 128 + (((ch & 7) ^ (lane & 7)) << 4)) =
               make_uint4(w[0], w[1], w[2], w[3]);
@@ -399,12 +469,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
           if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + ch * 8) = x;
         }
       }
+      }
       tc_fence_before_sync();
     } else if (warp < S::kMmaWarp) {
       const int dw = warp - S::kDequantWarp0;
       // lane i < KT / 16 has the page of block i of a tile; fetched a tile before it is needed
       auto fetch_pages = [&](int j) -> int {
-        const int key = j * KT + lane * kKv4Tokens, blk = key / kKv4Tokens;
+        const int key = (first + j) * KT + lane * kKv4Tokens, blk = key / kKv4Tokens;
         if (lane >= KT / kKv4Tokens || key >= len) return -1;
         const int page = table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
         if (page < 0 || page >= p.num_pages) {
@@ -415,7 +486,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       };
       // block `at` of tile j (for key `at` < len); null: no key, or its page does not exist
       auto block_at = [&](int pages, int j, int at) -> const uint8_t* {
-        const int page = __shfl_sync(0xffffffffu, pages, at), blk = j * (KT / kKv4Tokens) + at;
+        const int page = __shfl_sync(0xffffffffu, pages, at), blk = (first + j) * (KT / kKv4Tokens) + at;
         if (page < 0 || page >= p.num_pages) return nullptr;
         const int inner = p.page_shift >= 0 ? blk & (p.page_blocks - 1) : blk % p.page_blocks;
         return p.cache + ((static_cast<int64_t>(page) * p.kv_heads + h) * p.page_blocks + inner) * kBlock;
@@ -467,7 +538,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       const int hh = id % kHalves, eight = id / kHalves;  // half of the head, eight tokens
       uint32_t vw[4][nw], vpar[8][kGroups];
       auto load_values = [&](int j, int pages) {
-        const int key = j * KT + eight * 8;
+        const int key = (first + j) * KT + eight * 8;
         const uint8_t* blk = block_at(pages, j, eight >> 1);
         const int p0 = (eight & 1) * 4;  // first pair of tokens in its block
 #pragma unroll
@@ -602,14 +673,18 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
   }
 }
 
+// tiles of rows times kv heads, at most
+int64_t prompt_items(int batch, int64_t tokens, int heads, int kv_heads, int d) {
+  return (ceil_div(tokens * heads, d == 256 ? 128 : 256) + batch) * kv_heads;
+}
+
 template <typename T, int D, int G>
 cudaError_t launch_one(const Kv4AttendParams& p, cudaStream_t stream) {
   using S = Shape<D>;
   auto kernel = kv4_prompt_kernel<T, D, G>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total)) return e;
   cudaLaunchConfig_t cfg = {};
-  const int64_t tiles = ceil_div(static_cast<int64_t>(p.tokens) * p.heads, S::kRows) + p.batch;
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * p.kv_heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(prompt_items(p.batch, p.tokens, p.heads, p.kv_heads, D) * p.splits));
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::total;
   cfg.stream = stream;
@@ -638,6 +713,17 @@ cudaError_t launch_shape(const Kv4AttendParams& p, int d, int g, cudaStream_t st
 }
 
 }  // namespace
+
+// CTAs that share a tile of rows: as many as there are SMs for, where the cache can hold four tiles of keys for each.
+// (100 tokens of 32 heads behind 5000 cached ones: 24 tiles of rows at most.)
+int kv4_prompt_splits(int batch, int64_t tokens, int heads, int kv_heads, int d, int64_t max_keys, int num_sms) {
+  const int64_t by_sms = num_sms / prompt_items(batch, tokens, heads, kv_heads, d), by_keys = max_keys / (4 * (d == 256 ? 64 : 128));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({by_sms, by_keys, 16})));
+}
+size_t kv4_prompt_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms) {
+  const int64_t items = prompt_items(batch, tokens, heads, kv_heads, d);
+  return items * 2 > num_sms ? 0 : static_cast<size_t>(num_sms) * (d == 256 ? 1 : 2) * 128 * (d + 2) * 4;
+}
 
 cudaError_t launch_kv4_prompt(const Kv4AttendParams& p, int f16, int d, int g, cudaStream_t stream) {
   return f16 ? launch_shape<Kv4Fp16>(p, d, g, stream) : launch_shape<Kv4Bf16>(p, d, g, stream);

@@ -245,6 +245,34 @@ def test_prompts(ipex, d, heads, group, t, lens, new, causal):
     check(c, lens, new, heads, 60, causal=causal)
 
 
+@pytest.mark.parametrize("t", [BF, FP])
+@pytest.mark.parametrize("d, heads, lens, new", [
+    (128, 4, [5000, 700], [70, 33]), (64, 8, [3001], [64]), (256, 2, [2000, 40], [100, 1]), (128, 16, [900, 0, 1500], [5, 6, 20]),
+    (128, 4, [2500], [2500])])
+def test_short_prompts_behind_long_prefixes(ipex, t, d, heads, lens, new):
+    """Several CTAs share a tile of rows: parts that see nothing of a tile, a tile without rows, and the same bits again."""
+    c = cache_of(200, 1, d, 64, 32, t, fill=0xff)
+    got, table, q = check(c, lens, new, heads, 65)
+    starts = torch.tensor([0] + new).cumsum(0).int().cuda()
+    for _ in range(5):
+        assert torch.equal(c.attention(q.cuda(), table, torch.tensor(lens).int().cuda(), starts), got)
+
+
+@pytest.mark.parametrize("batch", [31, 257, 700])
+def test_shares_of_many_sequences(ipex, batch):
+    """More sequences than a warp, a CTA and a round of its warps look at; lengths all over, one long."""
+    lens = [(i * 37) % 90 for i in range(batch)]
+    lens[batch // 2] = 3000
+    c = cache_of(sum(-(-n // 16) for n in lens) + 1, 1, 64, 16, 64, BF, fill=0xff)
+    check(c, lens, [1] * batch, 4, 45, starts=False)
+
+
+def test_a_table_without_pages(ipex):
+    c = cache_of(3, 2, 64, 16, 32, BF)
+    o = c.attention(torch.ones(2, 4, 64).to(BF).cuda(), torch.zeros(2, 0).int().cuda(), torch.tensor([5, 0]).int().cuda())
+    assert (o == 0).all()
+
+
 def test_scores_of_any_size(ipex):
     """A scale of 0 is an average, a negative one turns the order round, wide keys make one token win."""
     c = cache_of(40, 2, 128, 16, 64, BF)
