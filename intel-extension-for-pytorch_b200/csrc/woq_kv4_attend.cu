@@ -23,7 +23,6 @@ constexpr int kWarps = 7;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kJoinBar = 1;
 constexpr int kMaxCtas = 512;
-constexpr int kMaxParts = 36;  // CTAs that share an item
 constexpr int kUnitKeys = 32;  // keys of a unit: two blocks
 
 // What an item costs beside its units (queries, joining the warps), in units: 222 units over 32 short sequences took
@@ -35,6 +34,9 @@ constexpr int kItemCost = 18;
 constexpr int ctas_per_sm(int d, int nt) { return nt * d <= 128 ? 2 : 1; }
 template <int D, int G, int NT>
 struct Smem {
+  // CTAs that share an item, what their statistics leave room for.  More of them are joined longer and read faster: one
+  // sequence of 100,000 tokens of one kv head takes 35.6 us with 36 CTAs, 26.4 with 64 and 23.6 with 112.
+  static constexpr int kMaxParts = NT > 2 ? 48 : 112;
   static constexpr int kCtas = ctas_per_sm(D, NT), kBlock = kv4_block_bytes(D, G);
   static constexpr size_t kBudget = kCtas == 2 ? 112 * 1024 : 226 * 1024;
   static constexpr size_t join = 0;                              // [kWarps][D][8] sums of the values
@@ -46,7 +48,8 @@ struct Smem {
   static constexpr size_t row_at = totals + 8 * NT * 8;          // [8 NT] places in the output
   static constexpr size_t full = row_at + 8 * NT * 8;            // [kWarps][kRing] barriers: the slot holds its block
   static constexpr size_t empty = full + kWarps * 8 * 8;         // the warp has read it
-  static constexpr size_t left_out = empty + kWarps * 8 * 8;     // words: nothing was loaded
+  static constexpr size_t weight = empty + kWarps * 8 * 8;       // [kMaxParts][8 NT] of the parts of an item
+  static constexpr size_t left_out = weight + kMaxParts * 8 * NT * 4;  // words: nothing was loaded
   static constexpr size_t ring = left_out + kWarps * 8 * 4;
   static constexpr int kFit = static_cast<int>((kBudget - ring) / (kWarps * kBlock)), kRing = kFit >= 8 ? 8 : kFit;
   static constexpr size_t total = ring + static_cast<size_t>(kWarps) * kRing * kBlock;
@@ -120,6 +123,7 @@ __device__ __forceinline__ void advance(const Kv4AttendParams& p, Cursor& c, int
 template <typename T, int D, int G, int NT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kernel(const __grid_constant__ Kv4AttendParams p) {
   using S = Smem<D, G, NT>;
+  constexpr int kMaxParts = S::kMaxParts;
   constexpr int kRows = 8 * NT, kRing = S::kRing, kBlock = S::kBlock, W = kv4_width(D), nw = W / 32, kHalves = D / W;
   constexpr int ng = D / G, kGroups = ng / kHalves, kWordsPerGroup = G / 32, kMt = D / 16;
   constexpr bool kQInRegs = S::kQInRegs;
@@ -176,11 +180,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
       s_run[warp][2] = longest;
     }
   }
-  __syncthreads();
+  const int runs = (p.batch + run - 1) / run;
+  if (runs > 1)
+    __syncthreads();
+  else
+    __syncwarp();  // (the first warp has them all)
   if (warp == 0) {
     int64_t total = 0, longest = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
+    for (int w = 0; w < runs; ++w) {
       total += s_run[w][0];
       longest = max(longest, s_run[w][2]);
     }
@@ -193,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
       auto locate = [&](int64_t place, int64_t& item_begin, int& b_out, int& item_out) -> int64_t {
         int64_t before = 0, before_units = 0;  // of the sequences before b0
         int b0 = 0;
-        for (int w = 0; w + 1 < kThreads / 32 && before + s_run[w][0] <= place; ++w) {
+        for (int w = 0; w + 1 < runs && before + s_run[w][0] <= place; ++w) {
           before += s_run[w][0];
           before_units += s_run[w][1];
           b0 += run;
@@ -232,8 +239,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
       if (end < total) {
         units += locate(end, unused, unused_b, unused_in);
       } else {
-#pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) units += s_run[w][1];
+        for (int w = 0; w < runs; ++w) units += s_run[w][1];
       }
       if (lane == 0) {
         s_b = b;
@@ -547,6 +553,18 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
         if (at >= 0) p.out[at + d] = T::from_float(l == 0.f ? 0.f : __fdividef(r[e], l) * Dequant<T>::kBack);
       }
     };
+    auto add_warps = [&](int i) {  // element i / 2, rows 4 (i & 1) to + 3
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(join + w * D * 8 + i * 4);
+        v.x += x.x;
+        v.y += x.y;
+        v.z += x.z;
+        v.w += x.w;
+      }
+      return v;
+    };
     // eight rows at a time: every warp's sums against the rows' common maximum, added in the order of the warps
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -595,17 +613,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
         if (!whole) *reinterpret_cast<float2*>(part + 2 * (nt * 8 + threadIdx.x)) = make_float2(m, l);
       }
       named_bar_sync(kJoinBar, kWarps * 32);
-      for (int i = threadIdx.x; i < D * 2; i += kWarps * 32) {  // element i / 2, four rows
+      for (int i = threadIdx.x; i < D * 2; i += kWarps * 32) {
         const int d = i / 2, row0 = (i & 1) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(join + w * D * 8 + i * 4);
-          v.x += x.x;
-          v.y += x.y;
-          v.z += x.z;
-          v.w += x.w;
-        }
+        const float4 v = add_warps(i);
         if (whole) {
           store(nt * 8 + row0, d, v);
         } else {
@@ -633,8 +643,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
         // (the item begins in its first CTA's share and before all others')
         auto part_of = [&](int c) { return p.partials + (2 * (first + c) + (c == 0)) * kPartial; };
         float2* ps = reinterpret_cast<float2*>(join);               // [part][row]
-        float* weight = join + 2 * kMaxParts * kRows;               // [part][row]
-        static_assert(3 * kMaxParts * kRows * 4 <= S::kJoinBytes, "joining buffer");
+        float* weight = reinterpret_cast<float*>(smem + S::weight);  // [part][row]
+        static_assert(2 * kMaxParts * kRows * 4 <= S::kJoinBytes, "joining buffer");
         for (int i = threadIdx.x; i < parts * kRows; i += kWarps * 32)
           ps[i] = __ldcg(reinterpret_cast<const float2*>(part_of(i / kRows)) + i % kRows);
         named_bar_sync(kJoinBar, kWarps * 32);
@@ -657,25 +667,32 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
           if (sub == 0) totals[row] = make_float2(m, l);
         }
         named_bar_sync(kJoinBar, kWarps * 32);
-        for (int i = threadIdx.x; i < D * 2 * NT; i += kWarps * 32) {
-          const int d = i / (2 * NT), row0 = i % (2 * NT) * 4;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int c0 = 0; c0 < parts; c0 += 4) {
-            float4 x[4];
+        // a warp adds every seventh part, all of it in flight; then the warps as above
+#pragma unroll 1
+        for (int nt = 0; nt < NT; ++nt) {
+          float4 v[kMt];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              x[k] = __ldcg(reinterpret_cast<const float4*>(part_of(min(c0 + k, parts - 1)) + 2 * kRows) + i);
+          for (int k = 0; k < kMt; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+          for (int c = warp; c < parts; c += kWarps) {
+            const float4 f = *reinterpret_cast<const float4*>(weight + c * kRows + nt * 8 + (lane & 1) * 4);
+            const float4* src = reinterpret_cast<const float4*>(part_of(c) + 2 * kRows + lane / 2 * kRows + nt * 8) + (lane & 1);
+            float4 x[kMt];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (c0 + k >= parts) break;
-              const float4 f = *reinterpret_cast<const float4*>(weight + (c0 + k) * kRows + row0);
-              v.x = fmaf(x[k].x, f.x, v.x);
-              v.y = fmaf(x[k].y, f.y, v.y);
-              v.z = fmaf(x[k].z, f.z, v.z);
-              v.w = fmaf(x[k].w, f.w, v.w);
+            for (int k = 0; k < kMt; ++k) x[k] = __ldcg(src + k * 4 * kRows);
+#pragma unroll
+            for (int k = 0; k < kMt; ++k) {
+              v[k].x = fmaf(x[k].x, f.x, v[k].x);
+              v[k].y = fmaf(x[k].y, f.y, v[k].y);
+              v[k].z = fmaf(x[k].z, f.z, v[k].z);
+              v[k].w = fmaf(x[k].w, f.w, v[k].w);
             }
           }
-          store(row0, d, v);
+#pragma unroll
+          for (int k = 0; k < kMt; ++k) *reinterpret_cast<float4*>(join + warp * D * 8 + (lane + 32 * k) * 4) = v[k];
+          named_bar_sync(kJoinBar, kWarps * 32);
+          for (int i = threadIdx.x; i < D * 2; i += kWarps * 32) store(nt * 8 + (i & 1) * 4, i / 2, add_warps(i));
+          if (nt + 1 < NT) named_bar_sync(kJoinBar, kWarps * 32);
         }
       }
     }
@@ -735,20 +752,26 @@ int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d) {
   return 4;
 }
 
-// Whether the prompt kernel takes a call: its tiles have 128 rows, the ones above 8, 16 or 32.
-bool kv4_attend_prompt(int batch, int64_t tokens, int heads) { return ceil_div(tokens, batch) * heads > 32; }
+// Whether the prompt kernel takes a call.  Its tiles have 128 rows, the ones above 8, 16 or 32, but its CTAs are long to
+// fill and to join.  With a tile for every SM it wins from the second small tile on (32 sequences of 1000 tokens, 8 kv
+// heads of 4 query heads and 128 elements, 9 new tokens: 54.8 us against 72.2), with fewer from about the fifth (one
+// sequence of 20,000 tokens: 12 new tokens 68 us against 37, 16 68 against 44, 32 68 against 76; 8 sequences of 2000: 16
+// new tokens 44.4 against 45.3, 24 44.7 against 62.1).  Elements of 64 and 256 divide alike.
+static bool kv4_attend_prompt(int batch, int64_t tokens, int heads, int kv_heads, int num_sms) {
+  return ceil_div(tokens, batch) * heads > (static_cast<int64_t>(batch) * kv_heads >= num_sms ? 32 : 64);
+}
 
 size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms) {
   const int nt = kv4_attend_tiles(batch, tokens, heads, d);
   const size_t few = static_cast<size_t>(ctas_for(nt, d, num_sms)) * 2 * 8 * nt * (d + 2) * 4;
-  return kv4_attend_prompt(batch, tokens, heads) ? std::max(few, kv4_prompt_partial_bytes(batch, tokens, heads, kv_heads, d, num_sms)) : few;
+  return kv4_attend_prompt(batch, tokens, heads, kv_heads, num_sms) ? std::max(few, kv4_prompt_partial_bytes(batch, tokens, heads, kv_heads, d, num_sms)) : few;
 }
 
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, int num_sms, cudaStream_t stream) {
   Kv4AttendParams q = p;
   q.page_shift = (p.page_blocks & (p.page_blocks - 1)) ? -1 : __builtin_ctz(static_cast<unsigned>(p.page_blocks));
   q.scale *= f16 ? Dequant<Kv4Fp16>::kBack : Dequant<Kv4Bf16>::kBack;
-  if (p.starts && kv4_attend_prompt(p.batch, p.tokens, p.heads)) {
+  if (p.starts && kv4_attend_prompt(p.batch, p.tokens, p.heads, p.kv_heads, num_sms)) {
     q.splits = kv4_prompt_splits(p.batch, p.tokens, p.heads, p.kv_heads, d, static_cast<int64_t>(p.max_blocks) * kKv4Tokens, num_sms);
     return launch_kv4_prompt(q, f16, d, g, stream);
   }

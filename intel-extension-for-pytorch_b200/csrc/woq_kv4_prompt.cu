@@ -387,10 +387,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         float* mine = p.partials + ((static_cast<int64_t>(item) * NQ + i) * p.splits + part) * kPart;
         *reinterpret_cast<float2*>(mine + 2 * r) = make_float2(top, sum);
 #pragma unroll 1
-        for (int c = 0; c < D / 32 && n > 0; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
           uint32_t x[32];
-          tmem_ld_x32(t_o + c * 32, x);
-          wait_ld_x32(x);
+          if (n > 0) {
+            tmem_ld_x32(t_o + c * 32, x);
+            wait_ld_x32(x);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = 0u;
+          }
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             *reinterpret_cast<uint4*>(mine + 256 + (c * 8 + e) * 512 + r * 4) = make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
@@ -427,12 +432,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         if (p.splits > 1) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) r[e] = 0u;
-#pragma unroll 1
+#pragma unroll 2
           for (int k = 0; k < p.splits; ++k) {
             const float* from = parts + k * kPart;
             const int rr = quarter * 32 + lane;
             const float2 st = __ldcg(reinterpret_cast<const float2*>(from + 2 * rr));
-            if (st.x == -INFINITY && st.y == 0.f) continue;  // saw nothing: its sums were not written
             const float f = st.x == -INFINITY ? 1.f : exp2_approx(st.x - top);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {

@@ -258,6 +258,25 @@ def test_short_prompts_behind_long_prefixes(ipex, t, d, heads, lens, new):
         assert torch.equal(c.attention(q.cuda(), table, torch.tensor(lens).int().cuda(), starts), got)
 
 
+@pytest.mark.parametrize("t", [BF, FP])
+@pytest.mark.parametrize("d, heads, new, length", [(128, 8, 1, 30000), (64, 1, 1, 26000), (256, 3, 2, 30001), (64, 16, 2, 20000)])
+def test_one_sequence_for_all(ipex, t, d, heads, new, length):
+    """One kv head of one sequence, so that as many CTAs share an item as may; the same bits again."""
+    c = cache_of(480, 1, d, 64, 32, t)
+    got, table, q = check(c, [length], [new], heads, 67)
+    starts = torch.tensor([0, new]).int().cuda()
+    for _ in range(5):
+        assert torch.equal(c.attention(q.cuda(), table, torch.tensor([length]).int().cuda(), starts), got)
+
+
+@pytest.mark.parametrize("batch, heads, new", [(3, 4, 16), (3, 4, 17), (200, 4, 8), (200, 4, 9), (200, 1, 33)])
+def test_where_the_tiles_of_rows_change(ipex, batch, heads, new):
+    """Numbers of rows around those from which tiles of 128 rows take a call, with few and with many sequences."""
+    c = cache_of(batch * 3, 1, 128, 32, 64, BF, fill=0xff)
+    lens = [(7 * b) % 60 + new - 5 for b in range(batch)]
+    check(c, lens, [new] * batch, heads, 68)
+
+
 @pytest.mark.parametrize("batch", [31, 257, 700])
 def test_shares_of_many_sequences(ipex, batch):
     """More sequences than a warp, a CTA and a round of its warps look at; lengths all over, one long."""
