@@ -651,11 +651,22 @@ cudaError_t launch_add_rmsnorm_quant(const __nv_bfloat16* x, int64_t ldx, const 
 #define ADD_NORM(CL, PIECES)                                                                                             \
   return asym ? launch_add_norm<true, CL, PIECES>(x, ldx, r, ldr, gamma, eps, m, k, sum, lds, qa, sa, zpa, stream)       \
               : launch_add_norm<false, CL, PIECES>(x, ldx, r, ldr, gamma, eps, m, k, sum, lds, qa, sa, zpa, stream)
+  // One CTA a row up to 6144 elements: a cluster's exchanges cost 0.7 us, more than the shorter row saves (1 x 4096 2.5 us
+  // against 3.2, 128 x 4096 3.3 against 5.9).  Longer rows are shared by a cluster while its CTAs find room at once: four
+  // with an SM each (1 x 8192 3.4 us against 3.7, 1 x 16384 4.1 against 6.4), two of the longest rows up to two an SM
+  // (256 x 14336 7.9 us against 10.1; 1024 x 14336 35.6 against 27.2).
+  const bool by_four = m * 4 <= 148, by_two = m * 2 <= 4 * 148;
   if (k <= kPer) ADD_NORM(1, 1);
-  if (m <= 128 && k <= 4 * kPer) ADD_NORM(4, 1);  // few rows: four CTAs each
   if (k <= 2 * kPer) ADD_NORM(1, 2);
-  if (k <= 4 * kPer) ADD_NORM(1, 4);
-  if (k <= 8 * kPer) ADD_NORM(1, 8);
+  if (k <= 4 * kPer) {
+    if (by_four && k > 3 * kPer) ADD_NORM(4, 1);
+    ADD_NORM(1, 4);
+  }
+  if (k <= 8 * kPer) {
+    if (by_four) ADD_NORM(4, 2);
+    if (by_two) ADD_NORM(2, 4);
+    ADD_NORM(1, 8);
+  }
   ADD_NORM(8, 8);
 #undef ADD_NORM
 }

@@ -60,6 +60,15 @@ def test_against_the_definition(ops, rows, k, asym):
     check(x, r, g, ops.woq_add_rmsnorm_quant(x, r, g, EPS, 2 if asym else 6), asym)
 
 
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("rows, k", [(37, 6160), (38, 6160), (37, 6144), (1, 8192), (37, 16384), (38, 8208), (296, 14336), (297, 14336)])
+def test_around_the_changes_of_the_split(ops, rows, k, asym):
+    gen = torch.Generator().manual_seed(rows + k)
+    x, r = torch.randn(rows, k, generator=gen).bfloat16().cuda(), (3 * torch.randn(rows, k, generator=gen)).bfloat16().cuda()
+    g = (1 + 0.3 * torch.randn(k, generator=gen)).bfloat16().cuda()
+    check(x, r, g, ops.woq_add_rmsnorm_quant(x, r, g, EPS, 2 if asym else 6), asym)
+
+
 def test_strides_shapes_and_types(ops):
     gen = torch.Generator().manual_seed(5)
     x = torch.randn(2, 3, 100, generator=gen).bfloat16().cuda()[..., 4:84]      # not aligned: copied
