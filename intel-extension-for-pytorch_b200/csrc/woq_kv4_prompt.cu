@@ -11,6 +11,10 @@
 // registers, one tile ahead; the dequantised values (bf16: times 2^-64, see Dequant) never leave the SM.
 // The running reference of the maximum is raised only when a score passes it by 8 (log2): P is at most 256 and O is
 // rescaled seldom.
+//
+// Bound by the softmax warps (two passes over the scores in tensor memory, an exponential an element) and, as much, by
+// the dequantising warps: each takes about 4100 cycles a tile of 256 x 128, whose products take 2048.  Prompts of 4096 and
+// 3000 tokens, 32 heads of 128 on 8, some behind cached ones: 344 us, 724 TFLOP/s.
 #include <algorithm>
 
 #include "woq_kernels.h"
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         tc_fence_after_sync();
       }
       // Parts of a row: {maximum, sum}, then its sums of values, four at a time, a row next to the other.  The last CTA adds
-      // them in the order of the keys.
+      // them in the order of the keys, two parts' sums on their way at a time.
       constexpr int kPart = 128 * (D + 2);
       const float* parts = p.partials + (static_cast<int64_t>(item) * NQ + i) * p.splits * kPart;
       if (p.splits > 1) {
@@ -424,55 +428,55 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
       }
       const float inv = sum == 0.f ? 0.f : Dequant<T>::kBack / sum;
       if (last) {
-      // to the place of the warp's query rows (their products are done) and from there, a row by D / 8 lanes
-      uint8_t* stage = smem + S::q + i * S::kQBytes + quarter * 32 * 128;
+        // to the place of the warp's query rows (their products are done) and from there, a row by D / 8 lanes
+        uint8_t* stage = smem + S::q + i * S::kQBytes + quarter * 32 * 128;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        if (p.splits > 1) {
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          if (p.splits > 1) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = 0u;
+            for (int e = 0; e < 32; ++e) r[e] = 0u;
 #pragma unroll 2
-          for (int k = 0; k < p.splits; ++k) {
-            const float* from = parts + k * kPart;
-            const int rr = quarter * 32 + lane;
-            const float2 st = __ldcg(reinterpret_cast<const float2*>(from + 2 * rr));
-            const float f = st.x == -INFINITY ? 1.f : exp2_approx(st.x - top);
+            for (int k = 0; k < p.splits; ++k) {
+              const float* from = parts + k * kPart;
+              const int rr = quarter * 32 + lane;
+              const float2 st = __ldcg(reinterpret_cast<const float2*>(from + 2 * rr));
+              const float f = st.x == -INFINITY ? 1.f : exp2_approx(st.x - top);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(from + 256 + (c * 8 + e) * 512 + rr * 4));
-              const float xs[4] = {x.x, x.y, x.z, x.w};
+              for (int e = 0; e < 8; ++e) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(from + 256 + (c * 8 + e) * 512 + rr * 4));
+                const float xs[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-              for (int q = 0; q < 4; ++q) r[4 * e + q] = __float_as_uint(fmaf(xs[q], f, __uint_as_float(r[4 * e + q])));
+                for (int q = 0; q < 4; ++q) r[4 * e + q] = __float_as_uint(fmaf(xs[q], f, __uint_as_float(r[4 * e + q])));
+              }
             }
+          } else if (n > 0) {
+            tmem_ld_x32(t_o + c * 32, r);
+            wait_ld_x32(r);
           }
-        } else if (n > 0) {
-          tmem_ld_x32(t_o + c * 32, r);
-          wait_ld_x32(r);
-        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t w[4];
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            w[k] = sum != 0.f ? T::pack(__uint_as_float(r[e * 8 + k * 2]) * inv, __uint_as_float(r[e * 8 + k * 2 + 1]) * inv) : 0u;
-          const int ch = c * 4 + e;
-          *reinterpret_cast<uint4*>(stage + (ch >> 3) * (128 * 128) + lane * 128 + (((ch & 7) ^ (lane & 7)) << 4)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
+            for (int k = 0; k < 4; ++k)
+              w[k] = sum != 0.f ? T::pack(__uint_as_float(r[e * 8 + k * 2]) * inv, __uint_as_float(r[e * 8 + k * 2 + 1]) * inv) : 0u;
+            const int ch = c * 4 + e;
+            *reinterpret_cast<uint4*>(stage + (ch >> 3) * (128 * 128) + lane * 128 + (((ch & 7) ^ (lane & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
-      }
-      __syncwarp();
-      {
-        const int64_t at = row < rows ? static_cast<int64_t>(q0 + token) * p.o_tok + static_cast<int64_t>(head) * p.o_head : -1;
-        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
+        __syncwarp();
+        {
+          const int64_t at = row < rows ? static_cast<int64_t>(q0 + token) * p.o_tok + static_cast<int64_t>(head) * p.o_head : -1;
+          constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;
 #pragma unroll 4
-        for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
-          const int r = r0 + lane / kLanes, ch = lane % kLanes;
-          const int64_t to = __shfl_sync(0xffffffffu, at, r);
-          const uint4 x = *reinterpret_cast<const uint4*>(stage + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-          if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + ch * 8) = x;
+          for (int r0 = 0; r0 < 32; r0 += kAtOnce) {
+            const int r = r0 + lane / kLanes, ch = lane % kLanes;
+            const int64_t to = __shfl_sync(0xffffffffu, at, r);
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+            if (to >= 0) *reinterpret_cast<uint4*>(p.out + to + ch * 8) = x;
+          }
         }
-      }
       }
       tc_fence_before_sync();
     } else if (warp < S::kMmaWarp) {
@@ -719,7 +723,9 @@ cudaError_t launch_shape(const Kv4AttendParams& p, int d, int g, cudaStream_t st
 }  // namespace
 
 // CTAs that share a tile of rows: as many as there are SMs for, where the cache can hold four tiles of keys for each.
-// (100 tokens of 32 heads behind 5000 cached ones: 24 tiles of rows at most.)
+// 100 tokens of 32 heads behind 5000 cached ones take 42.8 us with six CTAs a tile and 99.6 with one, 64 of 8 heads behind
+// 60,000 105 us against 1038.  Two tiles of keys for each: 200 tokens of 8 heads behind 3000 38.4 us against 35.6 with
+// four, 100 tokens of 32 heads behind 1000 27.6 against 29.8.
 int kv4_prompt_splits(int batch, int64_t tokens, int heads, int kv_heads, int d, int64_t max_keys, int num_sms) {
   const int64_t by_sms = num_sms / prompt_items(batch, tokens, heads, kv_heads, d), by_keys = max_keys / (4 * (d == 256 ? 64 : 128));
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({by_sms, by_keys, 16})));
