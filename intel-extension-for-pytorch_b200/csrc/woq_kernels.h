@@ -423,7 +423,7 @@ struct Kv4AttendParams {
   int* status;
   int64_t q_tok, q_head, o_tok, o_head, table_ld, num_pages;
   float scale;            // of the scores, times log2 e (below 2^63)
-  int batch, tokens, q_heads, kv_heads, heads;  // heads: query heads of a kv head
+  int batch, tokens, kv_heads, heads;  // heads: query heads of a kv head
   int page_blocks, max_blocks, causal;
   int page_shift;         // log2 of page_blocks, or -1 (set by the launch)
   int splits;             // prompts: CTAs that share a tile of rows (set by the launch)

@@ -164,8 +164,9 @@ int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const 
     return set_error(WOQ_B200_ERR_UNSUPPORTED, "a block table of %lld pages of %d tokens passes 2^31 tokens", (long long)max_pages,
                      d->page_size);
   const int heads = q_heads / d->kv_heads;
-  if (tokens > INT32_MAX / heads || static_cast<double>(batch) * d->kv_heads * (1.0 + max_pages * (d->page_size / 16.0)) *
-                                            (1.0 + static_cast<double>(tokens) * heads / 8) > 1e12)
+  // tiles of eight query rows, and their units of 32 keys (whose number in a CTA's share has 31 bits)
+  const double items = (static_cast<double>(tokens) * heads / 8 + static_cast<double>(batch)) * d->kv_heads;
+  if (tokens > INT32_MAX / heads || items > 2e9 || items * (20 + max_pages * (d->page_size / 32.0)) > 3e11)
     return set_error(WOQ_B200_ERR_UNSUPPORTED, "too many query rows and cached tokens for one call");
   if (!seq_lens || (max_pages > 0 && !block_table) || !workspace || (d->num_pages > 0 && !cache))
     return set_error(WOQ_B200_ERR_INVALID_ARG, "cache, block_table, seq_lens and workspace must be non-null");
@@ -199,7 +200,6 @@ int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const 
   p.scale = scale * 1.4426950408889634f;  // log2 e: the kernel's exponentials are powers of two
   p.batch = static_cast<int>(batch);
   p.tokens = static_cast<int>(tokens);
-  p.q_heads = q_heads;
   p.kv_heads = d->kv_heads;
   p.heads = heads;
   p.page_blocks = d->page_size / woq::kKv4Tokens;

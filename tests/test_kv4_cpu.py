@@ -83,6 +83,12 @@ def test_attention_calls_that_are_refused(capi, bad, code):
     assert attention(capi, **bad) == code
 
 
+def test_numbers_of_rows_that_no_launch_can_take(capi):
+    """Tiles of rows are numbered in 31 bits: many sequences for a few rows pass them as many rows do."""
+    assert attention(capi, starts=FAKE, batch=(1 << 31) - 1, tokens=1) == 2
+    assert attention(capi, starts=FAKE, batch=1, tokens=1 << 25, max_pages=1 << 23, table_ld=1 << 23) == 2
+
+
 def test_attention_of_nothing_is_fine(capi):
     assert attention(capi, batch=0, tokens=0, q=None, out=None, ws=None) == 0
 
