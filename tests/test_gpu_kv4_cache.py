@@ -269,6 +269,22 @@ def test_one_sequence_for_all(ipex, t, d, heads, new, length):
         assert torch.equal(c.attention(q.cuda(), table, torch.tensor([length]).int().cuda(), starts), got)
 
 
+@pytest.mark.parametrize("new", [1, 5, 70])
+def test_values_that_are_not_finite_in_a_shared_item(ipex, new):
+    """A token of the new ones that holds a NaN: rows before it keep their results, rows from it on are NaN, whichever CTA
+    had its keys.  One of the old ones: all rows are."""
+    c = cache_of(200, 1, 128, 64, 64, BF, fill=0xff)
+    got, table, q = check(c, [5000], [new], 4, 69)
+    starts, lens = torch.tensor([0, new]).int().cuda(), torch.tensor([5000]).int().cuda()
+    bad = torch.full((1, 1, 128), math.nan, dtype=BF, device="cuda")
+    for token in (5000 - 1 - new // 2, 2500):
+        slot = table[0, token // 64].long().reshape(1) * 64 + token % 64
+        c.append(torch.zeros_like(bad), bad, slot)
+        o = c.attention(q.cuda(), table, lens, starts)
+        first = max(0, token - (5000 - new))  # the first row that sees the token
+        assert torch.equal(o[:first], got[:first]) and o[first:].isnan().all()
+
+
 @pytest.mark.parametrize("batch, heads, new", [(3, 4, 16), (3, 4, 17), (200, 4, 8), (200, 4, 9), (200, 1, 33)])
 def test_where_the_tiles_of_rows_change(ipex, batch, heads, new):
     """Numbers of rows around those from which tiles of 128 rows take a call, with few and with many sequences."""
