@@ -253,6 +253,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
     hd->abort_flag = 0;
     hd->bad_page = 0;
   }
+  tc_fence_before_sync();
+  __syncthreads();
+  // Only now, with the tensor memory in hand: a dependent that allocates too and then waits for this grid must not find
+  // this CTA without it, since the two would wait for one another.
   grid_launch_dependents();
   grid_dependency_wait();
   const int part = blockIdx.x % p.splits, item = blockIdx.x / p.splits, h = item % p.kv_heads;
