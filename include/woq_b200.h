@@ -454,7 +454,8 @@ int woq_b200_kv4_read(const woq_b200_kv4_desc* desc, const void* cache, const in
                       void* v, void* stream);
 
 /* out = softmax(scale * q k^T) v over the cache.  Sequence b has seq_lens[b] cached tokens in the pages
- * block_table[b][0], [1], .. (rows table_ld entries apart; lengths beyond max_pages pages are cut) and the query
+ * block_table[b][0], [1], .. (rows table_ld entries apart; lengths beyond max_pages pages, at most 2^31 - 1024
+ * tokens, are cut) and the query
  * rows query_starts[b] .. query_starts[b + 1] - 1 (device array of batch + 1 entries; null: row b alone, and
  * tokens == batch).  `causal`: its queries are its last tokens, and a query does not see the tokens after it.
  * q_heads is a multiple of kv_heads; query head h reads kv head h / (q_heads / kv_heads).  A row that sees nothing is

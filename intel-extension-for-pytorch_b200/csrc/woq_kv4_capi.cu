@@ -160,13 +160,14 @@ int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const 
                      "sequences", (long long)tokens, (long long)batch);
   if (!(std::fabs(scale) < 1e18f)) return set_error(WOQ_B200_ERR_INVALID_ARG, "the scale must be a number below 1e18");
   if (tokens == 0 || batch == 0) return WOQ_B200_OK;
-  if (max_pages > 0 && (INT32_MAX - 15) / max_pages < d->page_size)
-    return set_error(WOQ_B200_ERR_UNSUPPORTED, "a block table of %lld pages of %d tokens passes 2^31 tokens", (long long)max_pages,
-                     d->page_size);
+  // (kernels number keys in 31 bits, up to three tiles of 128 and a warp of blocks behind the last one)
+  if (max_pages > 0 && (INT32_MAX - 1023) / max_pages < d->page_size)
+    return set_error(WOQ_B200_ERR_UNSUPPORTED, "a block table of %lld pages of %d tokens passes 2^31 - 1024 tokens",
+                     (long long)max_pages, d->page_size);
   const int heads = q_heads / d->kv_heads;
   // tiles of eight query rows, and their units of 32 keys (whose number in a CTA's share has 31 bits)
   const double items = (static_cast<double>(tokens) * heads / 8 + static_cast<double>(batch)) * d->kv_heads;
-  if (tokens > INT32_MAX / heads || items > 2e9 || items * (20 + max_pages * (d->page_size / 32.0)) > 3e11)
+  if (tokens > (INT32_MAX - 1023) / heads || items > 2e9 || items * (20 + max_pages * (d->page_size / 32.0)) > 3e11)
     return set_error(WOQ_B200_ERR_UNSUPPORTED, "too many query rows and cached tokens for one call");
   if (!seq_lens || (max_pages > 0 && !block_table) || !workspace || (d->num_pages > 0 && !cache))
     return set_error(WOQ_B200_ERR_INVALID_ARG, "cache, block_table, seq_lens and workspace must be non-null");
