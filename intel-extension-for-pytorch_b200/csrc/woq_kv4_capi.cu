@@ -34,6 +34,9 @@ int check_desc(const woq_b200_kv4_desc* d) {
   if (d->page_size <= 0 || d->page_size % woq::kKv4Tokens || d->kv_heads < 1 || d->kv_heads > 65535 || d->num_pages < 0)
     return set_error(WOQ_B200_ERR_INVALID_ARG, "the 4-bit cache needs a page size that is a multiple of 16, 1..65535 heads "
                      "and num_pages >= 0");
+  const int64_t page_bytes = static_cast<int64_t>(d->page_size / woq::kKv4Tokens) * woq::kv4_block_bytes(d->head_dim, d->group_size);
+  if (d->num_pages > INT64_MAX / d->kv_heads / page_bytes)
+    return set_error(WOQ_B200_ERR_INVALID_ARG, "the 4-bit cache's size passes 2^63 bytes");
   return WOQ_B200_OK;
 }
 

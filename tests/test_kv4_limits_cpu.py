@@ -34,3 +34,20 @@ def test_rows_that_do_not_leave_room_for_a_tile(capi):
     tokens = ((1 << 31) - 1) // 4
     assert capi.lib().woq_b200_kv4_attention(desc(capi), FAKE, FAKE, 0, 64, 4, FAKE, 4, 4, FAKE, FAKE, 1, tokens, 0.1, 1, FAKE,
                                              0, 64, FAKE, 1 << 40, None) == 2
+
+
+@pytest.mark.parametrize("over", [dict(num_pages=1 << 57), dict(num_pages=1 << 62), dict(num_pages=1 << 40, kv_heads=65535, page_size=1 << 20)])
+def test_caches_whose_bytes_pass_63_bits(capi, over):
+    """A size that wrapped round would be taken for the bytes to allocate."""
+    d, L = desc(capi, **over), capi.lib()
+    assert L.woq_b200_kv4_bytes(d) == 0
+    assert L.woq_b200_kv4_read(d, FAKE, FAKE, 1, FAKE, FAKE, None) == 1
+    assert L.woq_b200_kv4_append(d, FAKE, None, 0, 0, 0, FAKE, 64, 64, FAKE, 64, 64, FAKE, None, None, 0, 0, 0, 1, None, None) == 1
+    assert L.woq_b200_kv4_attention(d, FAKE, FAKE, 256, 64, over.get("kv_heads", 1), FAKE, 1, 1, FAKE, None, 1, 1, 0.1, 1, FAKE, 256,
+                                    64, FAKE, 1 << 40, None) == 1
+
+
+def test_a_cache_of_the_most_bytes_there_can_be(capi):
+    pages = ((1 << 63) - 1) // 1152
+    assert capi.lib().woq_b200_kv4_bytes(desc(capi, num_pages=pages)) == pages * 1152
+    assert capi.lib().woq_b200_kv4_bytes(desc(capi, num_pages=pages + 1)) == 0
