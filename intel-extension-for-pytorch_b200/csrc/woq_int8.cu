@@ -470,9 +470,12 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
   if (!(ss < INFINITY)) scale = __int_as_float(0x7fc00000);  // codes cannot say it: the row's scale does
   if (tid == 0 && slice == 0) sa[m] = scale;
   uint2* qr = reinterpret_cast<uint2*>(qa + m * k);
-  // The quotient by the scale's reciprocal is within 2^-15 of the true one; where that is near a tie the division decides.
-  // Adding 1.5 2^23 leaves the rounded code in the low bits.  (4096 x 8192: 54 us with divisions alone, 48 this way.)
+  // Codes by the scale's reciprocal; where that may be another than the division's, the division decides (4096 x 8192: 54 us
+  // with divisions alone, 48 this way).  Both quotients are off by at most 2^-23 and 2^-24 of themselves, and by 2^-17 each
+  // where a zero point is added.  A row far to one side of zero has quotients of up to 2^16 before the zero point, so the
+  // margin around a tie goes by the row's largest.  Adding 1.5 2^23 leaves the rounded code in the low bits.
   const float rcp = scale > 0.f ? __frcp_rn(scale) : 0.f;
+  const float clear = 0.5f - (fmaxf(fabsf(lo), fabsf(hi)) * rcp * (1.f / 4194304.f) + 1.f / 65536.f);
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int at = p0 + tid + i * 256;
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
       if (ASYM) t = fminf(fmaxf(t + zp, 0.f), 255.f);
       const float r = t + 12582912.f;
       c[j] = __float_as_uint(r);
-      near_tie = near_tie || fabsf(t - (r - 12582912.f)) > 0.4999f;
+      near_tie = near_tie || fabsf(t - (r - 12582912.f)) > clear;
     }
     if (near_tie && scale > 0.f) {
 #pragma unroll

@@ -1,0 +1,72 @@
+"""Codes of the residual's addition with RMS norm where the arithmetic is at its edges, exactly as the definition says.
+
+With every x + r equal to a power of two and eps = 0, the mean of the squares, its root and the normalised row are exact:
+y is the norm's weight, whatever it is.  Scale, zero point and codes then follow from 32-bit divisions alone."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    import ipex_b200
+
+    ipex_b200.load_ops()
+    return torch.ops.torch_ipex
+
+
+def quotient(a, b):
+    """a / b of fp32 numbers in fp32: 53 digits are more than twice 24 and two, so that rounding twice is rounding once."""
+    return (a.double() / b.double()).float()
+
+
+def definition(y, asym):
+    """y bf16 [k] (CPU) -> scale, zero point, codes, in 32-bit arithmetic."""
+    y = y.float()
+    if not asym:
+        s = quotient(y.abs().max(), torch.tensor(127.0))
+        return s, 0, quotient(y, s).round().clamp(-128, 127).int()
+    s = quotient(y.max() - y.min(), torch.tensor(255.0))
+    z = -quotient(y.min(), s).round()
+    return s, int(z), (quotient(y, s) + z).round().clamp(0, 255).int()
+
+
+def run(ops, y, asym, base=1.0, rows=1):
+    """The operator on rows whose normalised values are y."""
+    k = y.numel()
+    x = torch.full((rows, k), base / 2, device="cuda").bfloat16()
+    h, qa, sa, zpa = ops.woq_add_rmsnorm_quant(x, x, y.cuda(), 0.0, 2 if asym else 6)
+    assert (h == base).all()
+    codes = qa.view(torch.uint8) if asym else qa
+    return sa.cpu(), zpa.cpu(), codes.cpu().int()
+
+
+def check(ops, y, asym, base=1.0, rows=1):
+    sa, zpa, codes = run(ops, y, asym, base, rows)
+    s, z, c = definition(y, asym)
+    assert (sa == s).all() and (not asym or (zpa == z).all())
+    assert torch.equal(codes, c.expand(rows, -1))
+
+
+@pytest.mark.parametrize("rows, k", [(1, 64), (1, 8192), (150, 14336), (1, 16400), (3, 4112)])
+@pytest.mark.parametrize("low, sign", [(0.0, 1), (1.0, 1), (4.0, 1), (4.0, -1), (16.0, -1), (64.0, 1), (64.0, -1), (100.0, 1)])
+def test_rows_on_one_side(ops, rows, k, low, sign):
+    """Quotients of up to 2^15 before the zero point is added: neighbours in bf16 lie up to 255 codes apart, and many halfway
+    between two codes."""
+    gen = torch.Generator().manual_seed(int(low) + k)
+    for _ in range(4 if k > 64 else 60):
+        check(ops, (sign * (low + torch.rand(k, generator=gen))).bfloat16(), True, rows=rows)
+
+
+@pytest.mark.parametrize("asym", [False, True])
+def test_ties(ops, asym):
+    """Values at and next to every half code."""
+    for top in (127.0, 127.5, 254.0, 255.0, 63.5):
+        y = torch.arange(0, 256, 1).float() * 0.5 * (top / 127.5)
+        y = torch.cat((y, -y if not asym else y + 1.0, torch.tensor([top] + [0.0] * 15))).bfloat16()
+        check(ops, y, asym)
