@@ -473,9 +473,11 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
   // Codes by the scale's reciprocal; where that may be another than the division's, the division decides (4096 x 8192: 54 us
   // with divisions alone, 48 this way).  Both quotients are off by at most 2^-23 and 2^-24 of themselves, and by 2^-17 each
   // where a zero point is added.  A row far to one side of zero has quotients of up to 2^16 before the zero point, so the
-  // margin around a tie goes by the row's largest.  Adding 1.5 2^23 leaves the rounded code in the low bits.
+  // margin around a tie goes by the row's largest.  (Scales of up to 2^-128 have no finite reciprocal: nothing is clear then.)
+  // Adding 1.5 2^23 leaves the rounded code in the low bits.
   const float rcp = scale > 0.f ? __frcp_rn(scale) : 0.f;
-  const float clear = 0.5f - (fmaxf(fabsf(lo), fabsf(hi)) * rcp * (1.f / 4194304.f) + 1.f / 65536.f);
+  const float margin = fmaxf(fabsf(lo), fabsf(hi)) * rcp * (1.f / 4194304.f) + 1.f / 65536.f;
+  const float clear = rcp < INFINITY ? 0.5f - margin : -1.f;
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int at = p0 + tid + i * 256;
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
       if (ASYM) t = fminf(fmaxf(t + zp, 0.f), 255.f);
       const float r = t + 12582912.f;
       c[j] = __float_as_uint(r);
-      near_tie = near_tie || fabsf(t - (r - 12582912.f)) > clear;
+      near_tie = near_tie || !(fabsf(t - (r - 12582912.f)) <= clear);
     }
     if (near_tie && scale > 0.f) {
 #pragma unroll

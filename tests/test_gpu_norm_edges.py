@@ -70,3 +70,13 @@ def test_ties(ops, asym):
         y = torch.arange(0, 256, 1).float() * 0.5 * (top / 127.5)
         y = torch.cat((y, -y if not asym else y + 1.0, torch.tensor([top] + [0.0] * 15))).bfloat16()
         check(ops, y, asym)
+
+
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("power", [-133, -132, -130, -128, -126, -124, -120, -110])
+def test_scales_with_no_reciprocal(ops, asym, power):
+    """Rows whose largest value is so small that the scale's reciprocal passes the largest fp32 number."""
+    gen = torch.Generator().manual_seed(-power)
+    for spread in (1, 3, 100, 255):
+        y = (torch.randint(-spread, spread + 1, (64,), generator=gen).double() * 2.0 ** power).bfloat16()
+        check(ops, y, asym)
