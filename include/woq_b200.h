@@ -397,7 +397,8 @@ int woq_b200_rmsnorm_quant(const void* x, int64_t ldx, const void* gamma, float 
 
 /* The same behind a residual: sum = bf16(x + r) (the residual stream's new value), y = the RMSNorm of sum, and y's
  * codes, scales and zero points as above; y itself is not written.  `sum` may be x or r.  Rows of up to 131072
- * elements (k a multiple of 16).  A row whose sum of squares is not finite gets the scale NaN. */
+ * elements (k a multiple of 16).  A row whose sum of squares or range is not finite, or that has a y that is not, gets
+ * the scale NaN. */
 int woq_b200_add_rmsnorm_quant(const void* x, int64_t ldx, const void* r, int64_t ldr, const void* gamma, float eps,
                                int64_t m, int64_t k, int32_t act_quant_mode, void* sum, int64_t lds, void* qa, void* sa,
                                void* zpa, void* stream);

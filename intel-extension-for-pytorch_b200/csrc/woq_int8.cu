@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
   __syncthreads();
   const float inv = __frsqrt_rn(__fdiv_rn(ss, static_cast<float>(k)) + eps);
   float lo = INFINITY, hi = -INFINITY;
+  uint32_t most = 0;  // the largest magnitudes of y, as 16-bit numbers: minima and maxima leave NaN out
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int at = p0 + tid + i * 256;
@@ -440,11 +441,13 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
                                                      __uint_as_float(h[i][j] & 0xffff0000u) *
                                                          __uint_as_float(gw[j] & 0xffff0000u) * inv);
       h[i][j] = *reinterpret_cast<const uint32_t*>(&y);
+      most = __vmaxu2(most, h[i][j] & 0x7fff7fffu);
       const float a = __uint_as_float(h[i][j] << 16), b = __uint_as_float(h[i][j] & 0xffff0000u);
       lo = fminf(lo, fminf(a, b));
       hi = fmaxf(hi, fmaxf(a, b));
     }
   }
+  if ((most & 0xffffu) >= 0x7f80u || most >= 0x7f800000u) hi = INFINITY;
   block_min_max(lo, hi, red);
   if (CL > 1) {
     if (tid == 0) {
@@ -463,12 +466,14 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
   if (ASYM) {
     scale = __fdiv_rn(hi - lo, 255.0f);
     zp = -rintf(__fdiv_rn(lo, scale));
-    if (tid == 0 && slice == 0) zpa[m] = scale > 0.f ? static_cast<int32_t>(zp) : 0;
   } else {
     scale = __fdiv_rn(fmaxf(fabsf(hi), fabsf(lo)), 127.0f);
   }
-  if (!(ss < INFINITY)) scale = __int_as_float(0x7fc00000);  // codes cannot say it: the row's scale does
-  if (tid == 0 && slice == 0) sa[m] = scale;
+  if (!(ss < INFINITY) || !(scale < INFINITY)) scale = __int_as_float(0x7fc00000);  // codes cannot say it: the row's scale does
+  if (tid == 0 && slice == 0) {
+    if (ASYM) zpa[m] = scale > 0.f ? static_cast<int32_t>(zp) : 0;
+    sa[m] = scale;
+  }
   uint2* qr = reinterpret_cast<uint2*>(qa + m * k);
   // Codes by the scale's reciprocal; where that may be another than the division's, the division decides (4096 x 8192: 54 us
   // with divisions alone, 48 this way).  Both quotients are off by at most 2^-23 and 2^-24 of themselves, and by 2^-17 each

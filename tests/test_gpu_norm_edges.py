@@ -80,3 +80,14 @@ def test_scales_with_no_reciprocal(ops, asym, power):
     for spread in (1, 3, 100, 255):
         y = (torch.randint(-spread, spread + 1, (64,), generator=gen).double() * 2.0 ** power).bfloat16()
         check(ops, y, asym)
+
+
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows, k", [(1, 64), (1, 8192), (150, 14336), (2, 16400)])
+def test_weights_that_are_not_finite(ops, asym, bad, rows, k):
+    """A y that is not finite makes the row's scale NaN, wherever it stands."""
+    for at in (0, k // 2, k - 1):
+        y = torch.linspace(-1, 1, k).bfloat16()
+        y[at] = bad
+        assert run(ops, y, asym, rows=rows)[0].isnan().all()
