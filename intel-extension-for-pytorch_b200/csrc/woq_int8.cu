@@ -358,10 +358,10 @@ __global__ void __launch_bounds__(256) rmsnorm_quant_kernel(const __nv_bfloat16*
 }
 
 // The residual's addition, RMSNorm and the per-token quantiser: h = bf16(x + r), then what rmsnorm_quant_kernel does
-// on h.  A row is read once and stays in registers (PIECES of eight elements a thread, as bf16) from the sum to the
-// codes; CL CTAs of a cluster share a row and exchange their sums of squares and ranges through distributed shared
-// memory.  Bound by memory for many rows (7 bytes an element: 4096 x 8192 48 us, 4.9 TB/s), by one trip to memory and
-// two reductions of the CTA for few (1 x 4096 2.5 us).
+// on h, but for the order of the squares' sum and the root, which is rounded to nearest.  A row is read once and stays in
+// registers (PIECES of eight elements a thread, as bf16) from the sum to the codes; CL CTAs of a cluster share a row and
+// exchange their sums of squares and ranges through distributed shared memory.  Bound by memory for many rows (7 bytes an
+// element: 4096 x 8192 48 us, 4.9 TB/s), by one trip to memory and two reductions of the CTA for few (1 x 4096 2.5 us).
 __device__ __forceinline__ uint32_t add_bf16x2_rn(uint32_t a, uint32_t b) {
   const float lo = __uint_as_float(a << 16) + __uint_as_float(b << 16);
   const float hi = __uint_as_float(a & 0xffff0000u) + __uint_as_float(b & 0xffff0000u);
@@ -436,10 +436,10 @@ __global__ void __launch_bounds__(256) add_rmsnorm_quant_kernel(const __nv_bfloa
     const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      // (the product of two bf16 numbers is exact: one rounding in 32 bits less than h * inv * g)
-      const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(h[i][j] << 16) * __uint_as_float(gw[j] << 16) * inv,
-                                                     __uint_as_float(h[i][j] & 0xffff0000u) *
-                                                         __uint_as_float(gw[j] & 0xffff0000u) * inv);
+      // (h * inv first: at most the root of k, where h * g may pass the range of fp32 though y does not)
+      const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(h[i][j] << 16) * inv * __uint_as_float(gw[j] << 16),
+                                                     __uint_as_float(h[i][j] & 0xffff0000u) * inv *
+                                                         __uint_as_float(gw[j] & 0xffff0000u));
       h[i][j] = *reinterpret_cast<const uint32_t*>(&y);
       most = __vmaxu2(most, h[i][j] & 0x7fff7fffu);
       const float a = __uint_as_float(h[i][j] << 16), b = __uint_as_float(h[i][j] & 0xffff0000u);

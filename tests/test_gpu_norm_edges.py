@@ -91,3 +91,30 @@ def test_weights_that_are_not_finite(ops, asym, bad, rows, k):
         y = torch.linspace(-1, 1, k).bfloat16()
         y[at] = bad
         assert run(ops, y, asym, rows=rows)[0].isnan().all()
+
+
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("base, weight", [(2.0 ** 60, 2.0 ** 70), (2.0 ** -40, 2.0 ** -100)])
+def test_products_out_of_range_on_the_way(ops, asym, base, weight):
+    """y is in range though the sum times the weight, without the norm's factor, is not."""
+    gen = torch.Generator().manual_seed(3)
+    check(ops, (torch.randn(64, generator=gen) * weight).bfloat16(), asym, base)
+
+
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("low", [-1.0, 0.0, 3.0])
+def test_the_same_as_without_a_residual(ops, asym, low):
+    """Where the sums of squares are exact in any order, the operator and woq_rmsnorm_quant on the sum agree in every bit."""
+    gen = torch.Generator().manual_seed(4)
+    for k in (64, 2048, 4096):
+        x = torch.randint(-8, 9, (20, k), generator=gen).bfloat16().cuda()  # sums of squares below 2^24
+        r = torch.randint(-8, 9, (20, k), generator=gen).bfloat16().cuda()
+        g = (low + 2 * torch.rand(k, generator=gen)).bfloat16().cuda()
+        mode = 2 if asym else 6
+        h, qa, sa, zpa = ops.woq_add_rmsnorm_quant(x, r, g, 1e-5, mode)
+        qb, sb, zpb = ops.woq_rmsnorm_quant(h, g, 1e-5, mode)
+        # (the roots may differ in their last place: rows where they do have scales that do)
+        same = sa == sb
+        assert torch.equal(qa[same], qb[same])
+        assert not asym or torch.equal(zpa[same], zpb[same])
+        assert same.float().mean() > 0.9
