@@ -68,14 +68,16 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&c)[8],
   const uint16_t s16 = T::from_float_rz(__fdiv_rn(hi * 0.5f - lo * 0.5f, 7.5f));
   const float s = T::to_float(s16) * 0.5f, m = lo * 0.5f;
   // The quotient by the scale's reciprocal is within 2^-19 of the true one (two roundings of a number up to 15.2): where it
-  // is that near a tie, the division decides.  Adding 1.5 2^23 leaves the rounded quotient in the low bits.
+  // is that near a tie, the division decides, and everywhere for steps of up to 2^-127, whose halves have no finite
+  // reciprocal.  Adding 1.5 2^23 leaves the rounded quotient in the low bits.
   const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  const float clear = inv < INFINITY ? 0.5f - 1.f / 131072.f : -1.f;
   bool near_tie = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float t = fminf(fmaf(x[i], 0.5f, -m) * inv, 15.f), r = t + 12582912.f;
     c[i] = __float_as_uint(r) & 15u;
-    near_tie = near_tie || fabsf(t - (r - 12582912.f)) > 0.5f - 1.f / 131072.f;
+    near_tie = near_tie || !(fabsf(t - (r - 12582912.f)) <= clear);
   }
   if (near_tie && s > 0.f) {
 #pragma unroll
