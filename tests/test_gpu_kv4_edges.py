@@ -1,4 +1,7 @@
 """The 4-bit key/value cache where its arithmetic and its arguments are at their edges."""
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -45,3 +48,40 @@ def test_steps_with_no_reciprocal(ipex, t, power):
     x = (torch.randint(0, 256, (20, 1, 64), generator=torch.Generator().manual_seed(1)).double() * 2.0 ** power).to(t)
     x[:, :, 0] = 0  # (the lowest element of a group has code 0)
     assert torch.equal(stored(c, x), R.quantise(x, 32)[0])
+
+
+def digits(x, bits, how):
+    """A Fraction of normal size to a number of `bits` digits: toward zero (math.floor) or to the nearest, even (round)."""
+    if x == 0:
+        return x
+    e = math.frexp(float(abs(x)))[1]  # (of the number rounded to 64 bits: one too large just below a power of two)
+    e -= abs(x) < Fraction(2) ** (e - 1)
+    unit = Fraction(2) ** (e - bits)
+    return how(abs(x) / unit) * unit * (1 if x > 0 else -1)
+
+
+def quantised_exactly(row, t):
+    """One group in rational numbers: 64 bits do not hold the difference of a large and a tiny number."""
+    bits = 8 if t == BF else 11
+    x = [Fraction(float(v)) for v in row]
+    lo, hi = min(x), max(x)
+    s = digits((hi - lo) / 15, bits, math.floor)
+    return [digits(min(round((v - lo) / s), 15) * s + lo, bits, round) for v in x], s
+
+
+@pytest.mark.parametrize("t, low", [(BF, 2.0 ** -30), (BF, 2.0 ** -100), (FP, 2.0 ** -24), (BF, -2.0 ** -30), (FP, -2.0 ** -23)])
+def test_the_step_is_rounded_toward_zero_once(ipex, t, low):
+    """max - min just below (or above) 15 numbers of the type: 32 bits round it to all 15, the step is the number below."""
+    c = cache_of(1, 1, 64, 16, 64, t)
+    x = torch.zeros(6, 1, 64)
+    for i, top in enumerate((15.0, 7.5, 60.0, 30.0, 3.75, 120.0)):
+        x[i] = top * torch.linspace(0, 1, 64)
+        x[i, 0, 63], x[i, 0, 0] = top, low
+        x[i, 0, 1] = low
+    x = x.to(t)
+    got = stored(c, x)[:, 0].tolist()
+    for row, have in zip(x[:, 0], got):
+        want, s = quantised_exactly(row, t)
+        assert have[0] == want[0] == low and have[63] == want[63]
+        # codes of the others may lie on a border of two: a step apart at most there
+        assert all(abs(Fraction(h) - w) <= s for h, w in zip(have, want))
