@@ -532,9 +532,9 @@ int woq_b200_pair_plan(int32_t weight_dtype, int32_t columns, int64_t tiles, int
 /* The token columns woq_b200_linear_grouped takes for groups of these many rows (a diagnostic; needs no GPU). */
 int woq_b200_grouped_columns(const int64_t* rows, int32_t groups, int32_t* columns);
 
-/* Reads the status word of a workspace (synchronises the stream).  WOQ_B200_OK,
- * WOQ_B200_ERR_DEVICE_WAIT when a bounded wait inside a kernel gave up, or WOQ_B200_ERR_INVALID_ARG when
- * woq_b200_kv4_attention met a page that the cache does not have; the word is cleared. */
+/* Reads the status words of a workspace (synchronises the stream).  WOQ_B200_OK,
+ * WOQ_B200_ERR_DEVICE_WAIT when a bounded wait inside a kernel gave up, or else WOQ_B200_ERR_INVALID_ARG when
+ * woq_b200_kv4_attention met a page that the cache does not have; the words are cleared. */
 int woq_b200_workspace_status(void* workspace, void* stream);
 
 #ifdef __cplusplus

@@ -21,7 +21,7 @@ void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 namespace {
 
 constexpr uint64_t kMagic = 0x574f5142323030ull;  // "WOQB200"
-constexpr size_t kWsHeaderBytes = 64 * 1024;      // status word + per-tile arrival counters
+constexpr size_t kWsHeaderBytes = 64 * 1024;      // status words + per-tile arrival counters
 constexpr int kMaxCounterTiles = (kWsHeaderBytes - 256) / 4;
 
 thread_local char g_err[512] = "";
@@ -2095,15 +2095,17 @@ int woq_b200_grouped_columns(const int64_t* rows, int32_t groups, int32_t* colum
 int woq_b200_workspace_status(void* workspace, void* stream_) {
   if (!workspace) return fail(WOQ_B200_ERR_INVALID_ARG, "workspace is null");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  int h = 0;
-  CUDA_TRY(cudaMemcpyAsync(&h, workspace, sizeof(int), cudaMemcpyDeviceToHost, stream));
+  int h[2] = {0, 0};
+  static_assert(woq::kBadPageWord == 1, "the word behind the waits'");
+  CUDA_TRY(cudaMemcpyAsync(h, workspace, sizeof(h), cudaMemcpyDeviceToHost, stream));
   CUDA_TRY(cudaStreamSynchronize(stream));
-  if (h != 0) {
+  if (h[0] != 0 || h[1] != 0) {
     // a kernel that gave up may have left arrival counters behind: the whole header starts over
     CUDA_TRY(cudaMemsetAsync(workspace, 0, kWsHeaderBytes, stream));
-    if (h == woq::kStatusBadPage)
-      return fail(WOQ_B200_ERR_INVALID_ARG, "a block table named a page that the cache does not have: its keys were left out");
-    return fail(WOQ_B200_ERR_DEVICE_WAIT, "a bounded in-kernel wait gave up (code %d)", h);
+    if (h[0] != 0)
+      return fail(WOQ_B200_ERR_DEVICE_WAIT, "a bounded in-kernel wait gave up (code %d)%s", h[0],
+                  h[1] ? "; a block table also named a page that the cache does not have" : "");
+    return fail(WOQ_B200_ERR_INVALID_ARG, "a block table named a page that the cache does not have: its keys were left out");
   }
   return WOQ_B200_OK;
 }

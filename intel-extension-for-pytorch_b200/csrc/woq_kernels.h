@@ -434,7 +434,9 @@ cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, i
 int kv4_prompt_splits(int batch, int64_t tokens, int heads, int kv_heads, int d, int64_t max_keys, int num_sms);
 size_t kv4_prompt_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms);
 cudaError_t launch_kv4_prompt(const Kv4AttendParams& p, int f16, int d, int g, cudaStream_t stream);
-constexpr int kStatusBadPage = 901;  // a block table names a page that the cache does not have
+// Word of the workspace's header that says that a block table named a page that the cache does not have.  (The first word is
+// the waits' that were given up: the two do not stand in one another's way.)
+constexpr int kBadPageWord = 1;
 
 void count_launch();
 

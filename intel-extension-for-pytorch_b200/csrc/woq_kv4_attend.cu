@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
       if (go) {
         int page = next_page;
         if (page != kNone && (page < 0 || page >= p.num_pages)) {
-          atomicCAS(p.status, 0, kStatusBadPage);
+          p.status[kBadPageWord] = 1;
           page = kNone;
         }
         left_out[slot] = page == kNone;

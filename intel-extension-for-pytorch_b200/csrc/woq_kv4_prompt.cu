@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         const int page = table[p.page_shift >= 0 ? blk >> p.page_shift : blk / p.page_blocks];
         if (page < 0 || page >= p.num_pages) {
           *static_cast<volatile int*>(&hd->bad_page) = 1;
-          atomicCAS(p.status, 0, kStatusBadPage);
+          p.status[kBadPageWord] = 1;
         }
         return page;
       };

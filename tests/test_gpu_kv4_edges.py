@@ -1,4 +1,5 @@
 """The 4-bit key/value cache where its arithmetic and its arguments are at their edges."""
+import ctypes
 import math
 from fractions import Fraction
 
@@ -85,3 +86,35 @@ def test_the_step_is_rounded_toward_zero_once(ipex, t, low):
         assert have[0] == want[0] == low and have[63] == want[63]
         # codes of the others may lie on a border of two: a step apart at most there
         assert all(abs(Fraction(h) - w) <= s for h, w in zip(have, want))
+
+
+def test_a_wait_that_gave_up_is_reported_before_a_missing_page(ipex):
+    """Kernels record a wait that they gave up with a compare-and-swap on the first word of the workspace: a page that the
+    cache does not have, met before, must not stand in its way."""
+    from ipex_b200 import _capi
+
+    L = _capi.lib()
+    c = cache_of(4, 1, 64, 16, 64, BF)
+    x = randn(1, 16, 1, 64).to(BF).cuda()
+    c.append(x, x, torch.arange(16, device="cuda"))
+    d = _capi.Kv4Desc(4, 1, 64, 16, 64, _capi.T_BF16)
+    for new in (1, 80):  # both kernels
+        ws = torch.zeros(L.woq_b200_kv4_attention_workspace_bytes(ctypes.byref(d), 1, new, 4), dtype=torch.uint8, device="cuda")
+        q, out = randn(2, new, 4, 64).to(BF).cuda(), torch.zeros(new, 4, 64, dtype=BF, device="cuda")
+        table, lens, starts = torch.tensor([[0, 9]]).int().cuda(), torch.tensor([32]).int().cuda(), torch.tensor([0, new]).int().cuda()
+        stream = torch.cuda.current_stream().cuda_stream
+
+        def call():
+            assert L.woq_b200_kv4_attention(ctypes.byref(d), c.tensor.data_ptr(), q.data_ptr(), 256, 64, 4, table.data_ptr(), 2, 2,
+                                            lens.data_ptr(), starts.data_ptr(), 1, new, 0.125, 0, out.data_ptr(), 256, 64,
+                                            ws.data_ptr(), ws.numel(), stream) == 0
+
+        call()
+        assert L.woq_b200_workspace_status(ws.data_ptr(), stream) == 1 and b"page" in L.woq_b200_last_error()
+        assert L.woq_b200_workspace_status(ws.data_ptr(), stream) == 0 and not ws[:L.woq_b200_workspace_header_bytes()].any()
+        call()
+        first = ws[:4].view(torch.int32)
+        first.copy_(torch.where(first == 0, 910, first))  # what a kernel that gives up does
+        assert L.woq_b200_workspace_status(ws.data_ptr(), stream) == 6 and b"910" in L.woq_b200_last_error()
+        assert b"page" in L.woq_b200_last_error()
+        assert L.woq_b200_workspace_status(ws.data_ptr(), stream) == 0 and not ws[:L.woq_b200_workspace_header_bytes()].any()
