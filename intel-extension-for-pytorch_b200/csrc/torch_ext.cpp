@@ -613,6 +613,8 @@ at::Tensor kv4_index(const at::Tensor& t, const at::Tensor& cache, at::ScalarTyp
   TORCH_CHECK(t.device() == cache.device() && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong), "WOQ: ", what,
               " must be a tensor of int32 or int64 on the cache's device");
   if (t.scalar_type() == dtype && t.is_contiguous()) return t;
+  // (a number of 64 bits must not wrap to a page or length that there is)
+  if (dtype == at::kInt && t.scalar_type() == at::kLong) return t.clamp(INT32_MIN, INT32_MAX).to(dtype).contiguous();
   return t.to(dtype).contiguous();
 }
 at::Tensor kv4_empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& cache) {

@@ -118,3 +118,26 @@ def test_a_wait_that_gave_up_is_reported_before_a_missing_page(ipex):
         assert L.woq_b200_workspace_status(ws.data_ptr(), stream) == 6 and b"910" in L.woq_b200_last_error()
         assert b"page" in L.woq_b200_last_error()
         assert L.woq_b200_workspace_status(ws.data_ptr(), stream) == 0 and not ws[:L.woq_b200_workspace_header_bytes()].any()
+
+
+def test_numbers_of_64_bits_do_not_wrap(ipex):
+    """int64 tables, lengths and starts: a page of 2^32 + 1 is none that the cache has, a length of 2^32 + 5 is cut to the
+    table, negative ones stay negative."""
+    c = cache_of(4, 1, 64, 16, 64, BF)
+    x = randn(1, 64, 1, 64).to(BF)
+    c.append(x.cuda(), x.cuda(), torch.arange(64, device="cuda"))
+    kv = R.quantise(x, 64)[0]
+    q = randn(2, 3, 4, 64).to(BF)
+    table = torch.tensor([[0, (1 << 32) + 1, 2], [3, 2, -(1 << 32)], [1, 0, 1 << 62]]).cuda()
+    lens = torch.tensor([48, (1 << 32) + 5, 5 - (1 << 40)]).cuda()
+    torch.ops.torch_ipex.woq_check_status()
+    for starts, rows in ((None, [1, 1, 1]), (torch.tensor([-(1 << 33), 2, 3, (1 << 32) + 2]).cuda(), [2, 1, 0])):
+        got = c.attention(q.cuda(), table, lens, starts, causal=False).cpu().double()
+        with pytest.raises(RuntimeError, match="page"):
+            torch.ops.torch_ipex.woq_check_status()
+        row = 0
+        for n, keys in zip(rows, (list(range(16)) + list(range(32, 48)), list(range(48, 64)) + list(range(32, 48)), [])):
+            want, tol = R.attend(q[row:row + n].double(), kv[keys], kv[keys], 0.125, False)
+            assert ((got[row:row + n] - want).abs() <= tol(R.EPS[BF])).all()
+            row += n
+    torch.ops.torch_ipex.woq_check_status()
