@@ -461,7 +461,8 @@ int woq_b200_kv4_read(const woq_b200_kv4_desc* desc, const void* cache, const in
  * tokens == batch).  `causal`: its queries are its last tokens, and a query does not see the tokens after it.
  * q_heads is a multiple of kv_heads; query head h reads kv head h / (q_heads / kv_heads).  A row that sees nothing is
  * zeros (scales are below 1e18; bf16 keys and values below 2^-62 lose digits); rows of `out` that belong to no sequence stay as they are.  Lengths, tables and starts are read on the
- * device: a captured call follows them.  Workspace as for woq_b200_linear (its header zero before the first use).
+ * device: a captured call follows them.  Workspace as for woq_b200_linear (its header zero before the first use);
+ * one made for some sequences and rows serves every call of as many or fewer.
  * Keys of pages that the cache does not have are left out, and woq_b200_workspace_status then returns
  * WOQ_B200_ERR_INVALID_ARG.  Two calls with the same arguments give the same bits. */
 size_t woq_b200_kv4_attention_workspace_bytes(const woq_b200_kv4_desc* desc, int64_t batch, int64_t tokens,

@@ -430,6 +430,7 @@ struct Kv4AttendParams {
 };
 int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d);
 size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms);
+size_t kv4_attend_partial_bytes_up_to(int64_t tokens, int heads, int kv_heads, int d, int num_sms);
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, int num_sms, cudaStream_t stream);
 int kv4_prompt_splits(int batch, int64_t tokens, int heads, int kv_heads, int d, int64_t max_keys, int num_sms);
 size_t kv4_prompt_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms);

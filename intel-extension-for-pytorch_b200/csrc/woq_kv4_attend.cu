@@ -763,14 +763,29 @@ int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d) {
 // heads of 4 query heads and 128 elements, 9 new tokens: 54.8 us against 72.2), with fewer from about the fifth (one
 // sequence of 20,000 tokens: 12 new tokens 68 us against 37, 16 68 against 44, 32 68 against 76; 8 sequences of 2000: 16
 // new tokens 44.4 against 45.3, 24 44.7 against 62.1).  Elements of 64 and 256 divide alike.
+static int64_t kv4_small_tile_rows(int batch, int kv_heads, int num_sms) {
+  return static_cast<int64_t>(batch) * kv_heads >= num_sms ? 32 : 64;
+}
 static bool kv4_attend_prompt(int batch, int64_t tokens, int heads, int kv_heads, int num_sms) {
-  return ceil_div(tokens, batch) * heads > (static_cast<int64_t>(batch) * kv_heads >= num_sms ? 32 : 64);
+  return ceil_div(tokens, batch) * heads > kv4_small_tile_rows(batch, kv_heads, num_sms);
+}
+
+static size_t few_rows_bytes(int nt, int d, int num_sms) {
+  return static_cast<size_t>(ctas_for(nt, d, num_sms)) * 2 * 8 * nt * (d + 2) * 4;
 }
 
 size_t kv4_attend_partial_bytes(int batch, int64_t tokens, int heads, int kv_heads, int d, int num_sms) {
-  const int nt = kv4_attend_tiles(batch, tokens, heads, d);
-  const size_t few = static_cast<size_t>(ctas_for(nt, d, num_sms)) * 2 * 8 * nt * (d + 2) * 4;
+  const size_t few = few_rows_bytes(kv4_attend_tiles(batch, tokens, heads, d), d, num_sms);
   return kv4_attend_prompt(batch, tokens, heads, kv_heads, num_sms) ? std::max(few, kv4_prompt_partial_bytes(batch, tokens, heads, kv_heads, d, num_sms)) : few;
+}
+
+// The most that any call of up to `tokens` rows takes: a workspace made for a large call serves every smaller one.  (Large
+// calls share nothing between CTAs; of the prompts the fewest rows of one sequence are shared first.)
+size_t kv4_attend_partial_bytes_up_to(int64_t tokens, int heads, int kv_heads, int d, int num_sms) {
+  size_t most = 0;
+  for (int nt = 1; nt <= kv4_attend_tiles(1, tokens, heads, d); nt *= 2) most = std::max(most, few_rows_bytes(nt, d, num_sms));
+  const int64_t shortest = kv4_small_tile_rows(1, kv_heads, num_sms) / heads + 1;  // prompt
+  return tokens < shortest ? most : std::max(most, kv4_prompt_partial_bytes(1, shortest, heads, kv_heads, d, num_sms));
 }
 
 cudaError_t launch_kv4_attend(const Kv4AttendParams& p, int f16, int d, int g, int num_sms, cudaStream_t stream) {

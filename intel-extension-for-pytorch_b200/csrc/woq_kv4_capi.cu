@@ -144,7 +144,7 @@ size_t woq_b200_kv4_attention_workspace_bytes(const woq_b200_kv4_desc* d, int64_
   int sms = 0;
   if (num_sms(&sms) != WOQ_B200_OK) return 0;
   if (batch == 0 || tokens == 0) return partials_off();
-  return partials_off() + woq::kv4_attend_partial_bytes(static_cast<int>(batch), tokens, q_heads / d->kv_heads, d->kv_heads, d->head_dim, sms);
+  return partials_off() + woq::kv4_attend_partial_bytes_up_to(tokens, q_heads / d->kv_heads, d->kv_heads, d->head_dim, sms);
 }
 
 int woq_b200_kv4_attention(const woq_b200_kv4_desc* d, const void* cache, const void* q, int64_t q_tok, int64_t q_head,

@@ -141,3 +141,38 @@ def test_numbers_of_64_bits_do_not_wrap(ipex):
             assert ((got[row:row + n] - want).abs() <= tol(R.EPS[BF])).all()
             row += n
     torch.ops.torch_ipex.woq_check_status()
+
+
+@pytest.mark.parametrize("d, heads, kv_heads", [(64, 4, 8), (128, 4, 8), (256, 2, 4), (128, 1, 160), (64, 64, 1)])
+def test_a_workspace_serves_every_smaller_call(ipex, d, heads, kv_heads):
+    """Its size does not shrink with the sequences or the rows: a program makes one for its largest call."""
+    from ipex_b200 import _capi
+
+    L = _capi.lib()
+    desc = _capi.Kv4Desc(64, kv_heads, d, 16, 32, _capi.T_BF16)
+
+    def size(batch, tokens):
+        return L.woq_b200_kv4_attention_workspace_bytes(ctypes.byref(desc), batch, tokens, heads * kv_heads)
+
+    counts = [1, 2, 3, 5, 8, 9, 16, 17, 31, 33, 40, 64, 65, 100, 127, 128, 129, 255, 300, 1000, 4097, 20000]
+    for batch in (1, 2, 4, 7, 32, 100, 600):
+        sizes = [size(batch, n) for n in counts]
+        assert sizes == sorted(sizes), (batch, sizes)
+    for n in counts:
+        sizes = [size(batch, n) for batch in (1, 2, 4, 7, 32, 100, 600)]
+        assert sizes == sorted(sizes), (n, sizes)
+    # and the smaller calls are taken
+    ws = torch.zeros(size(4, 4000), dtype=torch.uint8, device="cuda")
+    cache = torch.zeros(L.woq_b200_kv4_bytes(ctypes.byref(desc)), dtype=torch.uint8, device="cuda")
+    for batch, n in ((1, 1), (4, 4), (3, 30), (1, 100), (4, 100), (1, 400), (4, 4000)):
+        q = torch.zeros(n, heads * kv_heads, d, dtype=BF, device="cuda")
+        out = torch.ones_like(q)
+        starts = (torch.arange(batch + 1, device="cuda") * (n // batch)).int()
+        table, lens = torch.arange(4, device="cuda").int().repeat(batch, 1), torch.full((batch,), 64, device="cuda").int()
+        rc = L.woq_b200_kv4_attention(ctypes.byref(desc), cache.data_ptr(), q.data_ptr(), q.stride(0), d, heads * kv_heads,
+                                      table.data_ptr(), 4, 4, lens.data_ptr(), starts.data_ptr(), batch, n, 0.1, 0, out.data_ptr(),
+                                      q.stride(0), d, ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, (batch, n, L.woq_b200_last_error())
+        torch.cuda.synchronize()
+        assert (out[:batch * (n // batch)] == 0).all()
+        assert L.woq_b200_workspace_status(ws.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
