@@ -5,7 +5,7 @@
 // CTAs in equal shares whatever the lengths; the warps of a CTA take its units in turn.  A warp computes S^T = K Q^T
 // and O^T += V^T P^T, so that up to eight query rows (the heads of a kv head, times tokens) fill the n side of
 // m16n8k16 and dequantised codes are A fragments as they come from the cache.  P^T is S^T transposed in registers
-// (movmatrix).  A running reference of the maximum is raised only when a score passes it by 8 (log2): P is at most 256.
+// (movmatrix).  The softmax's reference runs behind the maximum (woq_kv4_common.cuh).
 // When a tile of rows ends, the warps' sums are joined in shared memory; a tile that several CTAs share is joined
 // through the workspace by the last one, in a fixed order, so that results do not depend on who is last.
 //
@@ -460,13 +460,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(D, NT)) kv4_attend_kerne
         for (int e = 0; e < 2; ++e) m[e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
         const float over = fmaxf(m[0] - top[nt][0], m[1] - top[nt][1]);
         // (no score yet: -inf less -inf is NaN and stays; the first score is infinitely above)
-        if (__any_sync(0xffffffffu, over > 8.f)) {
+        if (__any_sync(0xffffffffu, over > T::kRaise)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 4));
             m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 8));
             m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 16));
-            m[e] = fmaxf(m[e], top[nt][e]);
+            m[e] = fmaxf(m[e] - T::kTopWeight, top[nt][e]);
             const float f = top[nt][e] == m[e] ? 1.f : exp2_approx(top[nt][e] - m[e]);
             top[nt][e] = m[e];
             sum[nt][e] *= f;

@@ -43,13 +43,18 @@ __host__ __device__ constexpr int kv4_value_half(int d, int r, int half, int j, 
   return 8 * d + half * w * 8 + (g * 8 + ((r >> 1) ^ kv4_swap(d, g))) * (nw * 4) + j * 4 + (r & 1) * 2;
 }
 
-// Arithmetic of the two 16-bit types
+// Arithmetic of the two 16-bit types.
+// Weights of the softmax are kept in the type as 2^(score - reference).  Any reference gives the same quotients; it is set
+// kTopWeight below the maximum and raised when a score passes it by kRaise, so that sums are seldom rescaled.  bf16 has room
+// below: weights of 1 to 2^8 at the top.  fp16 has none, and tens of thousands of small weights may be most of a result: 2^11
+// to 2^15 at the top, so that weights down to 2^-25 of the largest keep all their digits and down to 2^-35 some.
 struct Kv4Bf16 {
   using type = __nv_bfloat16;
   static constexpr bool kIsBf16 = true;
   static constexpr uint32_t kMagic = 0x43004300u;  // 128 + c with the code in the low bits
   static constexpr float kTooLarge = 2305843009213693952.f;  // 2^61: the attention kernel scales by 2^69
   static constexpr uint32_t kNan = 0x7fffu;
+  static constexpr float kTopWeight = 0.f, kRaise = 8.f;
   static __device__ __forceinline__ float to_float(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
   static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
   static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
@@ -80,6 +85,7 @@ struct Kv4Fp16 {
   static constexpr uint32_t kMagic = 0x64006400u;  // 1024 + c
   static constexpr float kTooLarge = INFINITY;
   static constexpr uint32_t kNan = 0x7fffu;
+  static constexpr float kTopWeight = 11.f, kRaise = 15.f;
   static __device__ __forceinline__ float to_float(uint16_t v) { return __half2float(__ushort_as_half(v)); }
   static __device__ __forceinline__ float lo(uint32_t v) { return to_float(static_cast<uint16_t>(v & 0xffffu)); }
   static __device__ __forceinline__ float hi(uint32_t v) { return to_float(static_cast<uint16_t>(v >> 16)); }

@@ -9,8 +9,7 @@
 //   1 warp                issues S = Q K^T and O += P V; allocates tensor memory
 // The products of one tile of rows run while the other tile's softmax does.  Codes are loaded straight into
 // registers, one tile ahead; the dequantised values (bf16: times 2^-64, see Dequant) never leave the SM.
-// The running reference of the maximum is raised only when a score passes it by 8 (log2): P is at most 256 and O is
-// rescaled seldom.
+// The softmax's reference runs behind the maximum (woq_kv4_common.cuh), so that O is rescaled seldom.
 //
 // Bound by the softmax warps (two passes over the scores in tensor memory, an exponential an element) and, as much, by
 // the dequantising warps: each takes about 4100 cycles a tile of 256 x 128, whose products take 2048.  Prompts of 4096 and
@@ -356,8 +355,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_prompt_kernel(const
         // read; the next 16 columns are on their way while the last ones are worked on
         float most = masked ? tile_max<KT, true>(t_s, sees - key0, gone) : tile_max<KT, false>(t_s, 0, 0);
         most *= scale;  // (NaN for a row that sees nothing of the tile at a scale of 0: ignored)
-        if (__any_sync(0xffffffffu, most - top > 8.f)) {
-          const float m = fmaxf(most, top), f = top == m ? 1.f : exp2_approx(top - m);
+        if (__any_sync(0xffffffffu, most - top > T::kRaise)) {
+          const float m = fmaxf(most - T::kTopWeight, top), f = top == m ? 1.f : exp2_approx(top - m);
           top = m;
           sum *= f;
           if (j > 0) {

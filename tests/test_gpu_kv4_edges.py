@@ -88,6 +88,29 @@ def test_the_step_is_rounded_toward_zero_once(ipex, t, low):
         assert all(abs(Fraction(h) - w) <= s for h, w in zip(have, want))
 
 
+@pytest.mark.parametrize("batch, heads, new, length", [(1, 4, 1, 60000), (300, 4, 1, 1000), (160, 2, 6, 1000), (1, 4, 70, 30000),
+                                                       (80, 4, 70, 1000)])
+@pytest.mark.parametrize("t", [BF, FP])
+def test_many_small_weights_beside_a_large_one(ipex, t, batch, heads, new, length):
+    """One key far above up to tens of thousands of others, each of 2^-25 of its weight: together they are the result, since the
+    large one's value is zero.  All sequences read the same pages; more of them leave more of the keys to one CTA."""
+    c = cache_of(-(-length // 64), 1, 64, 64, 64, t)
+    k, v = torch.zeros(length, 1, 64), 0.5 + torch.rand(length, 1, 64, generator=torch.Generator().manual_seed(2))
+    k[0, 0, 0], v[0] = 17.5, 0.0
+    k, v = k.to(t), v.to(t)
+    c.append(k.cuda(), v.cuda(), torch.arange(length, device="cuda"))
+    q = torch.zeros(batch * new, heads, 64)
+    q[..., 0] = 1.0
+    q = q.to(t)
+    table = torch.arange(c.num_pages, device="cuda").int().repeat(batch, 1)
+    starts = None if new == 1 else (torch.arange(batch + 1) * new).int().cuda()
+    lens = torch.full((batch,), length).int().cuda()
+    got = c.attention(q.cuda(), table, lens, starts, scale=1.0).cpu().double().unflatten(0, (batch, new))
+    want, tol = R.attend(q[:new].double(), R.quantise(k, 64)[0], R.quantise(v, 64)[0], 1.0, True)
+    assert want.abs().min() > 2.0 ** -17
+    assert ((got - want).abs() <= tol(R.EPS[t])).all()
+
+
 def test_a_wait_that_gave_up_is_reported_before_a_missing_page(ipex):
     """Kernels record a wait that they gave up with a compare-and-swap on the first word of the workspace: a page that the
     cache does not have, met before, must not stand in its way."""
