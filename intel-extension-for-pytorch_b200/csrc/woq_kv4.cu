@@ -65,9 +65,11 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&c)[8],
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  // Toward zero throughout, which is the true quotient's rounding: 15 times a number of T has at most 15 digits, so where the
-  // true range reaches it the range in 32 bits does.
-  const uint16_t s16 = T::from_float_rz(__fdiv_rz(__fsub_rz(hi * 0.5f, lo * 0.5f), 7.5f));
+  // Toward zero: 15 times a number of T has at most 15 digits, so the range in 32 bits, cut, reaches it where the true one does,
+  // and a quotient that was rounded up to a number of T is told by its product.
+  const float range = __fsub_rz(hi * 0.5f, lo * 0.5f);
+  uint16_t s16 = T::from_float_rz(__fdiv_rn(range, 7.5f));
+  if (T::to_float(s16) * 7.5f > range) --s16;
   const float s = T::to_float(s16) * 0.5f, m = lo * 0.5f;
   // The quotient by the scale's reciprocal is within 2^-19 of the true one (two roundings of a number up to 15.2): where it
   // is that near a tie, the division decides, and everywhere for steps of up to 2^-127, whose halves have no finite
