@@ -441,7 +441,7 @@ size_t woq_b200_kv4_bytes(const woq_b200_kv4_desc* desc);
  * [max_pos][rot], rot / 2 cosines then rot / 2 sines; pairs are (i, i + rot / 2), or (2 i, 2 i + 1) if `interleaved`.
  * Rotated keys are rounded to `dtype` before they are quantised.  q may be null with q_heads 0.
  * A slot outside the cache (-1 for padding) stores nothing; a position outside the table stores nothing either and
- * makes the token's q_out NaN.  The slots of one call must be distinct.  Where a head's key or value has an element
+ * makes the token's q_out NaN.  The slots of one call must be distinct.  Where a head's key (rotated) or value has an element
  * that is not finite (bf16: not below 2^61 in magnitude), the key reads back as NaN (and scores NaN) and a value with
  * such an element as zeros. */
 int woq_b200_kv4_append(const woq_b200_kv4_desc* desc, void* cache, const void* q, int64_t q_token_stride,
@@ -455,16 +455,21 @@ int woq_b200_kv4_read(const woq_b200_kv4_desc* desc, const void* cache, const in
                       void* v, void* stream);
 
 /* out = softmax(scale * q k^T) v over the cache.  Sequence b has seq_lens[b] cached tokens in the pages
- * block_table[b][0], [1], .. (rows table_ld entries apart; lengths beyond max_pages pages, at most 2^31 - 1024
- * tokens, are cut) and the query
- * rows query_starts[b] .. query_starts[b + 1] - 1 (device array of batch + 1 entries; null: row b alone, and
- * tokens == batch).  `causal`: its queries are its last tokens, and a query does not see the tokens after it.
+ * block_table[b][0], [1], .. (rows table_ld entries apart; lengths beyond max_pages pages, at most 2^31 - 1024 tokens,
+ * are cut) and the query rows query_starts[b] .. query_starts[b + 1] - 1 (device array of batch + 1 entries; null: row b
+ * alone, and tokens == batch).  `causal`: its queries are its last tokens, and a query does not see the tokens after it.
  * q_heads is a multiple of kv_heads; query head h reads kv head h / (q_heads / kv_heads).  A row that sees nothing is
- * zeros (scales are below 1e18; bf16 keys and values below 2^-62 lose digits); rows of `out` that belong to no sequence stay as they are.  Lengths, tables and starts are read on the
- * device: a captured call follows them.  Workspace as for woq_b200_linear (its header zero before the first use);
- * one made for some sequences and rows serves every call of as many or fewer.
- * Keys of pages that the cache does not have are left out, and woq_b200_workspace_status then returns
- * WOQ_B200_ERR_INVALID_ARG.  Two calls with the same arguments give the same bits. */
+ * zeros; rows of `out` that belong to no sequence stay as they are.  Lengths, tables and starts are read on the device: a
+ * captured call follows them.
+ * Scores, maxima and sums are held in 32 bits; the weights that meet the values are rounded to `dtype` once.  Scales are
+ * below 1e18; bf16 keys and values below 2^-62 lose digits.
+ * One kernel takes all sequences of a call, chosen by their rows on average.  Prompts and single tokens in one call give
+ * the right results, but take longer than a call each (64 sequences that decode behind 4096 tokens and a prompt of 1000:
+ * 367 us, apart 88 and 32).
+ * Workspace as for woq_b200_linear (its header zero before the first use); one made for some sequences and rows serves
+ * every call of as many or fewer.  Keys of pages that the cache does not have are left out, and
+ * woq_b200_workspace_status then returns WOQ_B200_ERR_INVALID_ARG.  Two calls with the same arguments give the same
+ * bits. */
 size_t woq_b200_kv4_attention_workspace_bytes(const woq_b200_kv4_desc* desc, int64_t batch, int64_t tokens,
                                               int32_t q_heads);
 int woq_b200_kv4_attention(const woq_b200_kv4_desc* desc, const void* cache, const void* q, int64_t q_token_stride,

@@ -94,9 +94,10 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&c)[8],
 }
 
 // One CTA per token (and part of its rows): D / 8 lanes a row, 8 elements a lane.  Rows are the query heads, then the
-// key heads, then the value heads; a thread keeps its 8 elements' angles over all rows.  Bound by the instructions of
-// rotation and quantiser at 32 warps an SM, the next round's loads under way meanwhile: 8000 tokens of 64 + 2 x 8 heads of
-// 128 92 us (3.4 TB/s of 6.6), 1001 of 25 + 2 x 5 heads of 64 7.6 us; few tokens by four trips to memory (8: 2.9 us).
+// key heads, then the value heads; a thread keeps its 8 elements' angles over all rows.  Bound by the latency of a CTA's trips
+// to memory (slot and position, angles, queries, keys and values), which 28 warps an SM do not cover: nearly half of the
+// stalls are waits for loads, 63 % of the issue slots are used, DRAM is at a third.  8000 tokens of 64 + 2 x 8 heads of 128
+// 93 us (3.3 TB/s of 6.6), 1001 of 25 + 2 x 5 heads of 64 7.7 us, 8 tokens 2.8 us.
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(256, 4) kv4_append_kernel(Kv4AppendParams p) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes, LG = G / 8, ng = D / G;
@@ -245,8 +246,9 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(Kv4AppendParams p) {
 }
 
 // One CTA per 16 listed slots and head (slots that follow one another share a block, whose sectors then come from
-// L1): D / 8 lanes a row.  Slots outside the cache give zeros.  Bound by the bytes that it writes: 8000 tokens of 8 heads
-// of 128 11 us.
+// L1): D / 8 lanes a row.  Slots outside the cache give zeros.  Bound by its instructions and the trips in front of them (a
+// value's eight codes come in eight loads of two bytes, behind the slot's): three quarters of the issue slots are used, the
+// bytes pass at 3.8 of 6.6 TB/s.  8000 tokens of 8 heads of 128 11 us.
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(256) kv4_read_kernel(Kv4ReadParams p) {
   constexpr int kLanes = D / 8, kRows = 256 / kLanes, LG = G / 8, ng = D / G;

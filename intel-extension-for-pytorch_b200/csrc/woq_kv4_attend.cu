@@ -9,10 +9,11 @@
 // When a tile of rows ends, the warps' sums are joined in shared memory; a tile that several CTAs share is joined
 // through the workspace by the last one, in a fixed order, so that results do not depend on who is last.
 //
-// Bound by the instructions of dequantiser and softmax (340 for a block of 16 keys, about 180 cycles of an SM), not by the
-// cache's bytes: 64 sequences of 1 to 8192 tokens, 64 heads of 128 on 8, 84 us = 3.6 TB/s of 6.6; two of 100,000 in fp16
-// 68 us.  Small calls are bound by what comes one after another (lengths, page numbers, blocks, joining warps and CTAs),
-// each part from a cold instruction cache: one sequence of 1025 tokens 10.8 us.
+// Bound by latency inside a warp's units (dequantise, products, maximum, exponentials, transpose, products, one behind the
+// other) at 14 computing warps an SM: about 350 instructions for a block of 16 keys at half of the issue slots, DRAM at 42 %.
+// 64 sequences of 1 to 8192 tokens, 64 heads of 128 on 8, 84 us = 3.6 TB/s of 6.6; two of 100,000 in fp16 68 us.  Small calls
+// are bound by what comes one after another (lengths, page numbers, blocks, joining warps and CTAs), each part from a cold
+// instruction cache: one sequence of 1025 tokens 10.8 us.
 #include <algorithm>
 
 #include "woq_kernels.h"
@@ -762,7 +763,9 @@ int kv4_attend_tiles(int batch, int64_t tokens, int heads, int d) {
 // fill and to join.  With a tile for every SM it wins from the second small tile on (32 sequences of 1000 tokens, 8 kv
 // heads of 4 query heads and 128 elements, 9 new tokens: 54.8 us against 72.2), with fewer from about the fifth (one
 // sequence of 20,000 tokens: 12 new tokens 68 us against 37, 16 68 against 44, 32 68 against 76; 8 sequences of 2000: 16
-// new tokens 44.4 against 45.3, 24 44.7 against 62.1).  Elements of 64 and 256 divide alike.
+// new tokens 44.4 against 45.3, 24 44.7 against 62.1).  Elements of 64 and 256 divide alike.  The rows are an average, since
+// lengths are not known here: 64 sequences of 4096 tokens with one new token each and a prompt of 1000 take 367 us in one call,
+// 88 and 32 in two.
 static int64_t kv4_small_tile_rows(int batch, int kv_heads, int num_sms) {
   return static_cast<int64_t>(batch) * kv_heads >= num_sms ? 32 : 64;
 }

@@ -118,3 +118,26 @@ def test_the_same_as_without_a_residual(ops, asym, low):
         assert torch.equal(qa[same], qb[same])
         assert not asym or torch.equal(zpa[same], zpb[same])
         assert same.float().mean() > 0.9
+
+
+@pytest.mark.parametrize("asym", [False, True])
+@pytest.mark.parametrize("rows, k", [(1, 64), (1, 8192), (40, 8192), (150, 14336), (2, 16400), (300, 4096)])
+def test_the_sum_in_the_place_of_an_operand(ops, rows, k, asym):
+    """The C entry writes the sum over x or over r, rows of any distance apart."""
+    from ipex_b200 import _capi
+
+    gen = torch.Generator().manual_seed(5)
+    x, r = (torch.randn(rows, k + 24, generator=gen).bfloat16().cuda() for _ in range(2))
+    g = torch.rand(k, generator=gen).bfloat16().cuda()
+    h, qa, sa, zpa = ops.woq_add_rmsnorm_quant(x[:, :k].contiguous(), r[:, :k].contiguous(), g, 1e-5, 2 if asym else 6)
+    for over in (0, 1):
+        a = [x.clone(), r.clone()]
+        behind = a[over][:, k:].clone()
+        codes, scales, zeros = torch.zeros_like(qa), torch.zeros_like(sa), torch.zeros(rows, dtype=torch.int32, device="cuda")
+        assert _capi.lib().woq_b200_add_rmsnorm_quant(a[0].data_ptr(), k + 24, a[1].data_ptr(), k + 24, g.data_ptr(), 1e-5, rows, k,
+                                                      2 if asym else 6, a[over].data_ptr(), k + 24, codes.data_ptr(), scales.data_ptr(),
+                                                      zeros.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert torch.equal(a[over][:, :k], h) and torch.equal(codes, qa) and torch.equal(scales, sa)
+        assert not asym or torch.equal(zeros, zpa)
+        assert torch.equal(a[over][:, k:], behind) and torch.equal(a[1 - over], (x, r)[1 - over])
