@@ -44,7 +44,8 @@ __host__ __device__ constexpr int kv4_value_half(int d, int r, int half, int j, 
 }
 
 // Arithmetic of the two 16-bit types.
-// Weights of the softmax are kept in the type as 2^(score - reference).  Any reference gives the same quotients; it is set
+// Weights of the softmax are kept in the type as 2^(score - reference), in one pass with a running maximum (Milakov and
+// Gimelshein, "Online normalizer calculation for softmax", 2018).  Any reference gives the same quotients; it is set
 // kTopWeight below the maximum and raised when a score passes it by kRaise, so that sums are seldom rescaled.  bf16 has room
 // below: weights of 1 to 2^8 at the top.  fp16 has none, and tens of thousands of small weights may be most of a result: 2^11
 // to 2^15 at the top, so that weights down to 2^-25 of the largest keep all their digits and down to 2^-35 some.
